@@ -389,6 +389,116 @@ int vaa_build_slot_mapping(const int32_t* block_table, int max_blocks_per_seq,
                            void* stream);
 
 /* ------------------------------------------------------------------------
+ * Quantised caches and sliding windows
+ * ---------------------------------------------------------------------- */
+
+/* How the K/V rows of a cache are held (vaa_kv_view.cache_type). */
+enum {
+  VAA_CACHE_16BIT = 0, /* 16-bit floats of vaa_attn_params.dtype */
+  VAA_CACHE_E4M3 = 1   /* e4m3 codes and one exponent byte a row */
+};
+
+/*
+ * How a cache is held and how much of it a query sees; no counterpart in the
+ * reference, which has 16-bit caches and whole contexts.
+ *
+ * VAA_CACHE_E4M3: a row (one token and kv head, head_size values) is head_size
+ * e4m3 codes c (the OCP format, largest value 448) in the cache and one byte b in
+ * key_exps / value_exps, and stands for the values c * 2^(b - 127).  The strides
+ * k_stride_*, v_stride_* of vaa_attn_params count codes (bytes), and the
+ * ke_/ve_stride_* here bytes of the exponents.  A written row has
+ *   z = the row with its magnitudes held to T, T = 61440 for fp16 and
+ *       15/16 * 2^128 for bf16 (so that what it stands for is finite; infinities
+ *       go to T, NaN to a NaN code),
+ *   e = the least integer with max|z| <= 448 * 2^e, at least -126,
+ *   c = z / 2^e rounded to nearest even,  b = e + 127.
+ *
+ * window, first_tokens: a query at position p sees the keys j <= p with
+ * j < first_tokens or j > p - window (its own key counts in the window);
+ * window = 0 is the whole context.  Keys that no query sees are not read, and
+ * their table entries may be anything.
+ */
+typedef struct vaa_kv_view {
+  int32_t cache_type;
+  int32_t window;
+  int32_t first_tokens;
+  int32_t reserved; /* 0 */
+  uint8_t* key_exps;
+  uint8_t* value_exps;
+  int64_t ke_stride_block, ke_stride_head, ke_stride_token;
+  int64_t ve_stride_block, ve_stride_head, ve_stride_token;
+} vaa_kv_view;
+
+/*
+ * vaa_kv_write_slots into a quantised cache: the rows new_keys / new_values
+ * (p->dtype, strides new_kv_stride_*) are rounded as above.  Any head_size; rows of
+ * at most 128 values, a multiple of 8, with 16-byte aligned 16-bit and 8-byte
+ * aligned code rows take the fast path.  Slots that name a row must differ: a slot
+ * named twice leaves its row unspecified.
+ */
+int vaa_kv_write_slots_q8(const vaa_attn_params* p, const vaa_kv_view* view, uint8_t* key_cache,
+                          uint8_t* value_cache, const void* slot_mapping, int slot_index_type,
+                          const uint16_t* new_keys, const uint16_t* new_values, int num_tokens,
+                          void* stream);
+
+/* vaa_kv_write_decode into a quantised cache. */
+int vaa_kv_write_decode_q8(const vaa_attn_params* p, const vaa_kv_view* view, uint8_t* key_cache,
+                           uint8_t* value_cache, const int32_t* block_table,
+                           const int32_t* seq_lens, const uint16_t* new_keys,
+                           const uint16_t* new_values, void* stream);
+
+/*
+ * The rows of a quantised cache that slot_mapping names, as 16-bit K and V of
+ * p->dtype at strides new_kv_stride_*: c * 2^(b - 127), rounded to the type (only
+ * values below fp16's normal range are).  Tokens without a slot (negative, or past
+ * the cache) get zeros.  Any slots, any number of times.
+ */
+int vaa_kv_read_slots_q8(const vaa_attn_params* p, const vaa_kv_view* view,
+                         const uint8_t* key_cache, const uint8_t* value_cache,
+                         const void* slot_mapping, int slot_index_type, uint16_t* keys,
+                         uint16_t* values, int num_tokens, void* stream);
+
+/*
+ * vaa_paged_attention_decode over a cache as `view` describes it: out[s, h, :] sums
+ * over the keys that position seq_lens[s] - 1 sees, which the cache already holds
+ * (there is no fused write).  Arguments, guards and workspace as there, with two
+ * differences: partition_size > 0 and the automatic one count the tokens that
+ * are seen, and VAA_PARTITION_BALANCED_SHARED is VAA_ERR_UNSUPPORTED.
+ * VAA_CACHE_E4M3: head_size a multiple of 16, codes 16-byte aligned with strides
+ * that are multiples of 16; K, Q and V enter the products as p->dtype, which holds
+ * every value of a row written from it exactly (fp16: but for those below its
+ * normal range).
+ */
+size_t vaa_paged_attention_decode_view_workspace_size(const vaa_attn_params* p,
+                                                      const vaa_kv_view* view,
+                                                      int32_t* partition_size_out);
+int vaa_paged_attention_decode_view(const vaa_attn_params* p, const vaa_kv_view* view,
+                                    const uint16_t* query, const void* key_cache,
+                                    const void* value_cache, const int32_t* block_table,
+                                    const int32_t* seq_lens, uint16_t* output, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/*
+ * vaa_paged_attention_prefill over a cache as `view` describes it: token t sees the
+ * keys that position positions[t] of sequence token_to_seq[t] sees.  Rows with an
+ * invalid sequence, a negative position or a context longer than the block table
+ * are left unwritten; keys in a missing block (id outside [0, num_blocks)) are not
+ * seen, as in the decode, and a row that sees none is zero.  Few query rows split
+ * the keys over workgroups and merge (a second launch); workspace:
+ * vaa_paged_attention_prefill_view_workspace_size bytes (0: none), 16-byte aligned,
+ * not shared by calls that can run concurrently.  p->max_seq_len bounds the
+ * contexts (it only sizes the split).  VAA_CACHE_E4M3 as for the decode.
+ */
+size_t vaa_paged_attention_prefill_view_workspace_size(const vaa_attn_params* p,
+                                                       const vaa_kv_view* view, int num_tokens);
+int vaa_paged_attention_prefill_view(const vaa_attn_params* p, const vaa_kv_view* view,
+                                     const uint16_t* query, const void* key_cache,
+                                     const void* value_cache, const int32_t* block_table,
+                                     const int32_t* token_to_seq, const int32_t* positions,
+                                     uint16_t* output, int num_tokens, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Layer ops next to attention.  `dtype` is VAA_DTYPE_F16 (the reference's
  * fp16) or VAA_DTYPE_BF16 for every 16-bit tensor of the call; arithmetic is
  * fp32, results round to nearest even.  Another value is VAA_ERR_UNSUPPORTED.

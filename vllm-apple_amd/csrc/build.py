@@ -34,6 +34,9 @@ SOURCES = [
     "topk.hip",
     "gate_up_silu.hip",
     "kv_stream.hip",
+    "kv_quant.hip",
+    "decode_view.hip",
+    "prefill_view.hip",
 ]
 
 ARCH = os.environ.get("VAA_OFFLOAD_ARCH", "gfx950")
@@ -44,11 +47,14 @@ ARCH = os.environ.get("VAA_OFFLOAD_ARCH", "gfx950")
 # the kernel is built without NaN semantics (infinities are kept): 3.5 %
 # faster on C3.
 #
-# The gate/up GEMM and the prefill issue their direct-to-LDS loads as inline
+# The prefill over a vaa_kv_view is built the same way, for the same reason.
+#
+# The gate/up GEMM and the prefills issue their direct-to-LDS loads as inline
 # asm that writes M0; clang warns that M0 is reserved because
 # compiler-generated code may use it (the asm declares it clobbered).
 FILE_FLAGS = {
     "paged_prefill.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
+    "prefill_view.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "gate_up_silu.hip": ["-Wno-inline-asm"],
 }
 

@@ -8,7 +8,7 @@
 // block/offset) that returns false to skip the token.  The new K/V rows are
 // read once, with the nontemporal hint (C3 chunk write 5.90 -> 5.67 us); the
 // cache rows are stored normally, since attention reads them next.
-#include "common.h"
+#include "kv_slots.h"
 
 namespace vaa {
 namespace {
@@ -24,42 +24,6 @@ struct NewSrc {
   const uint16_t* k;
   const uint16_t* v;
   int64_t s_tok, s_head;
-};
-
-// slot_mapping (kv_write.py:130-146): block = slot / bs, offset = slot % bs.
-template <typename IdxT>
-struct SlotResolver {
-  const IdxT* slots;
-  int block_size;
-  int64_t capacity;  // num_blocks * block_size
-  __device__ bool operator()(int t, int64_t& block, int64_t& off) const {
-    int64_t s = static_cast<int64_t>(slots[t]);
-    if (s < 0 || s >= capacity) return false;
-    block = s / block_size;
-    off = s % block_size;
-    return true;
-  }
-};
-
-// Decode position (paged_attention_fused.metal:73-86, kv_write.py:86-99).
-struct DecodeResolver {
-  const int32_t* block_table;
-  const int32_t* seq_lens;
-  int max_blocks_per_seq;
-  int block_size;
-  int64_t num_blocks;
-  __device__ bool operator()(int s, int64_t& block, int64_t& off) const {
-    int L = seq_lens[s];
-    if (L <= 0) return false;
-    int pos = L - 1;
-    int bi = pos / block_size;
-    if (bi >= max_blocks_per_seq) return false;
-    int phys = block_table[static_cast<int64_t>(s) * max_blocks_per_seq + bi];
-    if (phys < 0 || phys >= num_blocks) return false;
-    block = phys;
-    off = pos % block_size;
-    return true;
-  }
 };
 
 // Explicit (block id, offset) arrays (kv_write.c:50-57).  The reference

@@ -35,6 +35,9 @@ VAA_PARTITION_BALANCED_SHARED = -2
 # Element types of caches, queries, new K/V and outputs (vaa_attn_params.dtype).
 VAA_DTYPE_F16 = 0
 VAA_DTYPE_BF16 = 1
+# How a cache's rows are held (vaa_kv_view.cache_type).
+VAA_CACHE_16BIT = 0
+VAA_CACHE_E4M3 = 1
 ABI_VERSION = 6
 
 
@@ -77,11 +80,31 @@ class VaaAttnParams(ctypes.Structure):
     ]
 
 
+class VaaKvView(ctypes.Structure):
+    """Mirror of ``struct vaa_kv_view``."""
+
+    _fields_ = [
+        ("cache_type", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("first_tokens", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("key_exps", ctypes.c_void_p),
+        ("value_exps", ctypes.c_void_p),
+        ("ke_stride_block", ctypes.c_int64),
+        ("ke_stride_head", ctypes.c_int64),
+        ("ke_stride_token", ctypes.c_int64),
+        ("ve_stride_block", ctypes.c_int64),
+        ("ve_stride_head", ctypes.c_int64),
+        ("ve_stride_token", ctypes.c_int64),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _PARAMS = ctypes.POINTER(VaaAttnParams)
+_VIEW = ctypes.POINTER(VaaKvView)
 
 # name -> (restype, argtypes); must match include/vllm_apple_amd.h
 SIGNATURES = {
@@ -127,6 +150,16 @@ SIGNATURES = {
     "vaa_topk_logits": (_I, [_P, _I, _I, _I64, _I, _P, _P, _I64, _P, ctypes.c_size_t, _P]),
     "vaa_qkv_epilogue": (_I, [_PARAMS, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _I, _P, _P, _I,
                               _P]),
+    "vaa_kv_write_slots_q8": (_I, [_PARAMS, _VIEW, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "vaa_kv_write_decode_q8": (_I, [_PARAMS, _VIEW, _P, _P, _P, _P, _P, _P, _P]),
+    "vaa_kv_read_slots_q8": (_I, [_PARAMS, _VIEW, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "vaa_paged_attention_decode_view_workspace_size": (
+        ctypes.c_size_t, [_PARAMS, _VIEW, ctypes.POINTER(ctypes.c_int32)]),
+    "vaa_paged_attention_decode_view": (_I, [_PARAMS, _VIEW, _P, _P, _P, _P, _P, _P, _P,
+                                             ctypes.c_size_t, _P]),
+    "vaa_paged_attention_prefill_view_workspace_size": (ctypes.c_size_t, [_PARAMS, _VIEW, _I]),
+    "vaa_paged_attention_prefill_view": (_I, [_PARAMS, _VIEW, _P, _P, _P, _P, _P, _P, _P, _I, _P,
+                                              ctypes.c_size_t, _P]),
     "vaa_kv_stream_read": (_I, [_PARAMS, _P, _P, _P, _P, _P, _P]),
 }
 
@@ -164,7 +197,9 @@ def load() -> ctypes.CDLL:
                 f"ABI version mismatch: {_LIB_PATH} has {lib.vaa_abi_version()}, "
                 f"this package needs {ABI_VERSION} (rebuild the library)")
         for name, (res, args) in SIGNATURES.items():
-            fn = getattr(lib, name)
+            fn = getattr(lib, name, None)
+            if fn is None:
+                raise NativeLibraryError(f"{_LIB_PATH} lacks {name} (rebuild the library)")
             fn.restype = res
             fn.argtypes = args
         try:

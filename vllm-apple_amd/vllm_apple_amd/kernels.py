@@ -9,9 +9,17 @@ KV caches are described by a layout name:
             (vllm_apple/metal/kv_cache.py:213-219)
   "vllm":   K = kv_cache[0], V = kv_cache[1], each [num_blocks, block_size,
             num_kv_heads, head_size] (metal_attn.py:171-185)
+
+A quantised cache is a pair of such tensors of torch.float8_e4m3fn codes and, for
+each, a uint8 tensor of its shape without the last dimension, the rows' exponent
+bytes (key_exps, value_exps): code c of a row with byte b stands for c * 2^(b - 127)
+(vaa_kv_view in include/vllm_apple_amd.h).  kv_write_slots, kv_write_decode,
+paged_decode and paged_prefill take them beside the codes; kv_read_slots gives rows
+back.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -89,8 +97,9 @@ def make_params(*, key_cache: torch.Tensor, value_cache: torch.Tensor, layout: s
                 num_query_heads: int, scale: float, num_seqs: int = 0,
                 max_seq_len: int = 0, max_blocks_per_seq: int = 0,
                 query: torch.Tensor | None = None, output: torch.Tensor | None = None,
-                new_kv: torch.Tensor | None = None,
-                partition_size: int = 0) -> _lib.VaaAttnParams:
+                new_kv: torch.Tensor | None = None, partition_size: int = 0,
+                dtype: torch.dtype | None = None) -> _lib.VaaAttnParams:
+    """dtype: the 16-bit type beside a quantised cache (default: the caches')."""
     ks = cache_strides(key_cache, layout)
     vs = cache_strides(value_cache, layout)
     if (ks.num_blocks, ks.block_size, ks.num_kv_heads, ks.head_size) != (
@@ -99,11 +108,13 @@ def make_params(*, key_cache: torch.Tensor, value_cache: torch.Tensor, layout: s
     if num_query_heads % ks.num_kv_heads != 0:
         raise ValueError(
             f"num_query_heads={num_query_heads} not a multiple of num_kv_heads={ks.num_kv_heads}")
-    if key_cache.dtype != value_cache.dtype or key_cache.dtype not in ATTN_DTYPES:
+    if dtype is None:
+        dtype = key_cache.dtype
+    if key_cache.dtype != value_cache.dtype or dtype not in ATTN_DTYPES:
         raise ValueError(f"caches must both be float16 or bfloat16, got "
                          f"{key_cache.dtype}/{value_cache.dtype}")
     p = _lib.VaaAttnParams()
-    p.dtype = ATTN_DTYPES[key_cache.dtype]
+    p.dtype = ATTN_DTYPES[dtype]
     p.scale = float(scale)
     p.num_seqs = int(num_seqs)
     p.max_seq_len = int(max_seq_len)
@@ -132,13 +143,22 @@ def make_params(*, key_cache: torch.Tensor, value_cache: torch.Tensor, layout: s
 
 def kv_write_slots(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
                    value_cache: torch.Tensor, slot_mapping: torch.Tensor, *,
+                   key_exps: torch.Tensor | None = None, value_exps: torch.Tensor | None = None,
                    layout: str = "kernel", stream=None) -> None:
     """cache[slot // bs, :, slot % bs] = key/value[t] for every slot >= 0.
 
     key/value: [num_tokens, num_kv_heads, head_size] fp16 or bf16 (any token/head
     strides with a contiguous last dim); slot_mapping: int32 or int64
     [num_tokens].  Mirrors kv_write.py:118-156 and base_attn.py:308-342.
+
+    key_exps, value_exps: the caches are quantised, and the rows are rounded to e4m3
+    codes with a power-of-two scale each (vaa_kv_write_slots_q8); slots that name a
+    row must then differ.
     """
+    if key_exps is not None or value_exps is not None:
+        _rows_call("vaa_kv_write_slots_q8", key, value, key_cache, value_cache, key_exps,
+                   value_exps, slot_mapping, layout, stream)
+        return
     if key.is_cuda and layout in _IS_VLLM and _lib.host().kv_write(
             key, value, key_cache, value_cache, slot_mapping, _IS_VLLM[layout],
             _lib.stream_handle(stream)) is True:
@@ -164,8 +184,32 @@ def kv_write_slots(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tens
 
 def kv_write_decode(new_keys: torch.Tensor, new_values: torch.Tensor, key_cache: torch.Tensor,
                     value_cache: torch.Tensor, block_table: torch.Tensor,
-                    seq_lens: torch.Tensor, *, layout: str = "kernel", stream=None) -> None:
-    """Write each sequence's new token at position seq_lens[s]-1 (kv_write.py:66-114)."""
+                    seq_lens: torch.Tensor, *, key_exps: torch.Tensor | None = None,
+                    value_exps: torch.Tensor | None = None, layout: str = "kernel",
+                    stream=None) -> None:
+    """Write each sequence's new token at position seq_lens[s]-1 (kv_write.py:66-114);
+    with key_exps and value_exps into a quantised cache, rounded as by kv_write_slots."""
+    if key_exps is not None or value_exps is not None:
+        dev = _one_device(new_keys=new_keys, new_values=new_values, key_cache=key_cache,
+                          value_cache=value_cache, key_exps=key_exps, value_exps=value_exps,
+                          block_table=block_table, seq_lens=seq_lens)
+        dt = _attn_dtype(new_keys=new_keys, new_values=new_values)
+        view = _kv_view(key_cache, value_cache, key_exps, value_exps, layout)
+        _check_tables(block_table, seq_lens)
+        num_seqs = seq_lens.numel()
+        p = make_params(key_cache=key_cache, value_cache=value_cache, layout=layout,
+                        num_query_heads=cache_strides(key_cache, layout).num_kv_heads, scale=1.0,
+                        num_seqs=num_seqs, max_blocks_per_seq=block_table.shape[1],
+                        new_kv=new_keys, dtype=dt)
+        _check_rows(new_keys, new_values, p, "new_keys and new_values")
+        if new_keys.shape[0] < num_seqs:
+            raise ValueError("new_keys has fewer rows than sequences")
+        with _on_device(dev):
+            _lib.call("vaa_kv_write_decode_q8", ctypes.byref(p), ctypes.byref(view),
+                      key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+                      seq_lens.data_ptr(), new_keys.data_ptr(), new_values.data_ptr(),
+                      _lib.stream_handle(stream))
+        return
     _require_gpu(new_keys, new_values, key_cache, value_cache, block_table, seq_lens)
     _attn_dtype(new_keys=new_keys, new_values=new_values, key_cache=key_cache,
                 value_cache=value_cache)
@@ -427,7 +471,9 @@ def paged_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
                  max_seq_len: int, layout: str = "kernel", output: torch.Tensor | None = None,
                  new_keys: torch.Tensor | None = None, new_values: torch.Tensor | None = None,
                  partition_size: int = 0, workspace: torch.Tensor | None = None,
-                 seq_lens_host=None, shared: bool = False, stream=None) -> torch.Tensor:
+                 seq_lens_host=None, shared: bool = False, stream=None, window: int = 0,
+                 first_tokens: int = 0, key_exps: torch.Tensor | None = None,
+                 value_exps: torch.Tensor | None = None) -> torch.Tensor:
     """Paged GQA decode attention, one query token per sequence.
 
     query [num_seqs, H, D] fp16 or bf16 (the caches', new K/V's and output's
@@ -442,7 +488,23 @@ def paged_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     overlap): an automatic balanced split then uses PARTITION_BALANCED_SHARED,
     half-size workgroups, four per CU's worth of the split, that share CUs
     with the other kernel.
+
+    window > 0: the query, at position L - 1, sees the keys j with j < first_tokens or
+    j >= L - window only (its own key counts in the window); table entries of other
+    keys may be anything.  key_exps, value_exps: the caches are quantised.  Either
+    way (vaa_paged_attention_decode_view) the cache already holds the new token
+    (new_keys and new_values are refused), partition_size counts tokens that are
+    seen, and `shared` is a hint that changes nothing.
     """
+    if window or first_tokens or key_exps is not None or value_exps is not None:
+        if new_keys is not None or new_values is not None:
+            raise ValueError("new_keys/new_values: write the new token before a decode with a "
+                             "window or over a quantised cache")
+        return _decode_view(query, key_cache, value_cache, block_table, seq_lens, scale=scale,
+                            max_seq_len=max_seq_len, layout=layout, output=output,
+                            partition_size=partition_size, workspace=workspace,
+                            seq_lens_host=seq_lens_host, stream=stream, window=window,
+                            first_tokens=first_tokens, key_exps=key_exps, value_exps=value_exps)
     if query.is_cuda and output is not None and layout in _IS_VLLM and key_cache.dim() == 4 \
             and query.dim() == 3:
         part = partition_size
@@ -656,7 +718,9 @@ def paged_prefill(query: torch.Tensor, key_cache: torch.Tensor, value_cache: tor
                   positions: torch.Tensor, *, scale: float, layout: str = "kernel",
                   output: torch.Tensor | None = None, split_keys: int = 0,
                   max_seq_len: int = 0, workspace: torch.Tensor | None = None,
-                  stream=None, tiles: torch.Tensor | None = None) -> torch.Tensor:
+                  stream=None, tiles: torch.Tensor | None = None, window: int = 0,
+                  first_tokens: int = 0, key_exps: torch.Tensor | None = None,
+                  value_exps: torch.Tensor | None = None) -> torch.Tensor:
     """Chunked-prefill attention: token t attends to cache positions [0, positions[t]].
 
     query [num_tokens, H, D] fp16 or bf16, as the caches and output; the
@@ -668,7 +732,20 @@ def paged_prefill(query: torch.Tensor, key_cache: torch.Tensor, value_cache: tor
     max_seq_len bounds the contexts (default: the block table's capacity) and
     sizes the partials' workspace (grow-only scratch unless given).
     tiles: build_prefill_tiles' table for these tokens.
+
+    window > 0: token t sees the keys j <= p = positions[t] with j < first_tokens or
+    j > p - window only.  key_exps, value_exps: the caches are quantised.  Either way
+    (vaa_paged_attention_prefill_view) keys in a missing block are not seen instead
+    of leaving their rows unwritten, the call splits the keys by itself (split_keys
+    and tiles are refused) and max_seq_len only sizes that split.
     """
+    if window or first_tokens or key_exps is not None or value_exps is not None:
+        if split_keys or tiles is not None:
+            raise ValueError("split_keys and tiles do not go with a window or a quantised cache")
+        return _prefill_view(query, key_cache, value_cache, block_table, token_to_seq, positions,
+                             scale=scale, layout=layout, output=output, max_seq_len=max_seq_len,
+                             workspace=workspace, stream=stream, window=window,
+                             first_tokens=first_tokens, key_exps=key_exps, value_exps=value_exps)
     if query.is_cuda and output is not None and layout in _IS_VLLM \
             and (not split_keys or (max_seq_len and workspace is not None)) \
             and _lib.host().prefill(query, key_cache, value_cache, block_table, token_to_seq,
@@ -801,6 +878,242 @@ def build_slot_mapping(block_table: torch.Tensor, block_size: int, token_to_seq:
               token_to_seq.data_ptr(), positions.data_ptr(), block_table.shape[0], n,
               out.data_ptr(), _lib.stream_handle(stream))
     return out
+
+# ------------------------------------------- quantised caches, sliding windows
+
+QUANT_DTYPE = torch.float8_e4m3fn
+
+
+def _one_device(**named: torch.Tensor | None) -> torch.device:
+    """The GPU that all the given tensors are on."""
+    devices = {n: t.device for n, t in named.items() if t is not None}
+    kinds = set(devices.values())
+    if len(kinds) != 1 or next(iter(kinds)).type != "cuda":
+        raise ValueError(f"tensors must be on one ROCm device (there is no CPU fallback), got "
+                         f"{ {n: str(d) for n, d in devices.items()} }")
+    return next(iter(kinds))
+
+
+def _check_exps(cache: torch.Tensor, exps: torch.Tensor, name: str) -> None:
+    if cache.dtype != QUANT_DTYPE:
+        raise ValueError(f"{name} goes with a float8_e4m3fn cache, got {cache.dtype}")
+    if exps.dtype != torch.uint8 or exps.shape != cache.shape[:-1]:
+        raise ValueError(f"{name} must be uint8 {tuple(cache.shape[:-1])}, got {exps.dtype} "
+                         f"{tuple(exps.shape)}")
+
+
+def _kv_view(key_cache: torch.Tensor, value_cache: torch.Tensor,
+             key_exps: torch.Tensor | None, value_exps: torch.Tensor | None, layout: str,
+             window: int = 0, first_tokens: int = 0) -> _lib.VaaKvView:
+    """vaa_kv_view of a cache (checked with its exponents, if any)."""
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
+    if (key_exps is None) != (value_exps is None):
+        raise ValueError("key_exps and value_exps go together")
+    if not (0 <= window < 1 << 31 and 0 <= first_tokens < 1 << 31):
+        raise ValueError(f"window={window} and first_tokens={first_tokens} must be 0 or positive")
+    v = _lib.VaaKvView()
+    v.window, v.first_tokens = int(window), int(first_tokens)
+    if key_exps is None:
+        if QUANT_DTYPE in (key_cache.dtype, value_cache.dtype):
+            raise ValueError("a float8_e4m3fn cache needs key_exps and value_exps")
+        return v
+    _check_exps(key_cache, key_exps, "key_exps")
+    _check_exps(value_cache, value_exps, "value_exps")
+    h, t = (1, 2) if layout == "kernel" else (2, 1)
+    v.cache_type = _lib.VAA_CACHE_E4M3
+    v.key_exps, v.value_exps = key_exps.data_ptr(), value_exps.data_ptr()
+    v.ke_stride_block, v.ke_stride_head, v.ke_stride_token = (
+        key_exps.stride(0), key_exps.stride(h), key_exps.stride(t))
+    v.ve_stride_block, v.ve_stride_head, v.ve_stride_token = (
+        value_exps.stride(0), value_exps.stride(h), value_exps.stride(t))
+    return v
+
+
+def _on_device(device: torch.device):
+    """Makes the tensors' device the current one, where it is not."""
+    if _dev_index(device) == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_rows(key: torch.Tensor, value: torch.Tensor, p: _lib.VaaAttnParams,
+                names: str = "key and value") -> None:
+    if key.shape != value.shape or key.stride() != value.stride():
+        raise ValueError(f"{names} must have identical shapes and strides")
+    if tuple(key.shape[1:]) != (p.num_kv_heads, p.head_size):
+        raise ValueError(f"{names}: shape {tuple(key.shape)} does not match the cache")
+
+
+def _check_slots(slot_mapping: torch.Tensor, n: int) -> int:
+    """The VAA_INDEX_* code of a slot mapping for n tokens."""
+    if slot_mapping.dtype not in (torch.int32, torch.int64) or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous int32/int64 tensor")
+    if slot_mapping.numel() < n:
+        raise ValueError(f"slot_mapping has {slot_mapping.numel()} entries < {n} tokens")
+    return _lib.VAA_INDEX_I64 if slot_mapping.dtype == torch.int64 else _lib.VAA_INDEX_I32
+
+
+def _rows_call(name: str, key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+               value_cache: torch.Tensor, key_exps: torch.Tensor, value_exps: torch.Tensor,
+               slot_mapping: torch.Tensor, layout: str, stream) -> None:
+    """vaa_kv_write_slots_q8 or vaa_kv_read_slots_q8."""
+    dev = _one_device(key=key, value=value, key_cache=key_cache, value_cache=value_cache,
+                      key_exps=key_exps, value_exps=value_exps, slot_mapping=slot_mapping)
+    dt = _attn_dtype(key=key, value=value)
+    view = _kv_view(key_cache, value_cache, key_exps, value_exps, layout)
+    p = make_params(key_cache=key_cache, value_cache=value_cache, layout=layout,
+                    num_query_heads=cache_strides(key_cache, layout).num_kv_heads, scale=1.0,
+                    new_kv=key, dtype=dt)
+    _check_rows(key, value, p)
+    itype = _check_slots(slot_mapping, key.shape[0])
+    with _on_device(dev):
+        caches = (key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), itype)
+        _lib.call(name, ctypes.byref(p), ctypes.byref(view), *caches, key.data_ptr(),
+                  value.data_ptr(), key.shape[0], _lib.stream_handle(stream))
+
+
+def kv_read_slots(key_cache: torch.Tensor, value_cache: torch.Tensor, key_exps: torch.Tensor,
+                  value_exps: torch.Tensor, slot_mapping: torch.Tensor, *,
+                  dtype: torch.dtype = torch.float16, key: torch.Tensor | None = None,
+                  value: torch.Tensor | None = None, layout: str = "kernel",
+                  stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(key, value) [num_tokens, KV, D]: the rows of a quantised cache that
+    slot_mapping (int32 or int64) names, as values of dtype (fp16 or bf16; that of
+    key and value where they are given, which are then filled).  Tokens without a
+    slot (negative, or past the cache) get zeros."""
+    if (key is None) != (value is None):
+        raise ValueError("key and value go together")
+    if key is None:
+        cs = cache_strides(key_cache, layout)
+        shape = (slot_mapping.numel(), cs.num_kv_heads, cs.head_size)
+        dev = _one_device(key_cache=key_cache, slot_mapping=slot_mapping)
+        with _on_device(dev):
+            key, value = (_stream_empty(shape, dtype, dev, stream) for _ in range(2))
+    _rows_call("vaa_kv_read_slots_q8", key, value, key_cache, value_cache, key_exps, value_exps,
+               slot_mapping, layout, stream)
+    return key, value
+
+
+def _stream_empty(shape: tuple, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """A result of one call, from the caching allocator of the stream it runs on."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(_as_stream(stream, device)):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _as_stream(stream, device: torch.device) -> torch.cuda.Stream:
+    """A torch stream for what a wrapper takes: None, a torch stream, or anything with
+    a raw handle."""
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    return torch.cuda.ExternalStream(int(stream.cuda_stream), device=device)
+
+
+def _view_partition(seq_lens_host, query: torch.Tensor, num_kv_heads: int, window: int,
+                    first_tokens: int, quantised: bool) -> int:
+    """The split-K mode of a decode over a view from its host lengths: the choice for
+    the tokens that are seen, two quantised ones counted as one."""
+    lens = _int_tuple(seq_lens_host)
+    if window:
+        top = window + first_tokens
+        lens = tuple(min(n, top) for n in lens)
+    if quantised:
+        lens = tuple((n + 1) // 2 for n in lens)
+    part = _decode_partition(query, num_kv_heads, lens, False)
+    return 2 * part if quantised and part > 0 else part
+
+
+def _decode_view(query, key_cache, value_cache, block_table, seq_lens, *, scale, max_seq_len,
+                 layout, output, partition_size, workspace, seq_lens_host, stream, window,
+                 first_tokens, key_exps, value_exps) -> torch.Tensor:
+    """paged_decode over a quantised cache and/or with a sliding window."""
+    dev = _one_device(query=query, key_cache=key_cache, value_cache=value_cache,
+                      block_table=block_table, seq_lens=seq_lens, output=output,
+                      key_exps=key_exps, value_exps=value_exps, workspace=workspace)
+    view = _kv_view(key_cache, value_cache, key_exps, value_exps, layout, window, first_tokens)
+    q8 = key_exps is not None
+    rows = dict(query=query, output=output)
+    dt = _attn_dtype(**rows) if q8 else _attn_dtype(key_cache=key_cache, value_cache=value_cache,
+                                                    **rows)
+    _check_tables(block_table, seq_lens)
+    num_seqs = seq_lens.numel()
+    with _on_device(dev):
+        if output is None:
+            output = _stream_empty(tuple(query.shape), dt, dev, stream)
+        if query.shape[0] < num_seqs or output.shape[0] < num_seqs:
+            raise ValueError("query/output have fewer rows than sequences")
+        if output.dim() != 3 or output.shape[1:] != query.shape[1:]:
+            raise ValueError("output must have the query's heads and head_size")
+        if partition_size == 0 and seq_lens_host is not None:
+            partition_size = _view_partition(
+                seq_lens_host, query, cache_strides(key_cache, layout).num_kv_heads, window,
+                first_tokens, q8)
+        p = make_params(key_cache=key_cache, value_cache=value_cache, layout=layout,
+                        num_query_heads=query.shape[1], scale=scale, num_seqs=num_seqs,
+                        max_seq_len=max_seq_len, max_blocks_per_seq=block_table.shape[1],
+                        query=query, output=output, partition_size=partition_size, dtype=dt)
+        if query.shape[2] != p.head_size:
+            raise ValueError(f"query head_size {query.shape[2]} != cache head_size {p.head_size}")
+        nbytes = _lib.load().vaa_paged_attention_decode_view_workspace_size(
+            ctypes.byref(p), ctypes.byref(view), None)
+        ws = workspace if workspace is not None else _stream_scratch(nbytes, dev, stream)
+        _lib.call("vaa_paged_attention_decode_view", ctypes.byref(p), ctypes.byref(view),
+                  query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                  block_table.data_ptr(), seq_lens.data_ptr(), output.data_ptr(), _ptr(ws),
+                  ws.numel() * ws.element_size() if ws is not None else 0,
+                  _lib.stream_handle(stream))
+    return output
+
+
+def _prefill_view(query, key_cache, value_cache, block_table, token_to_seq, positions, *, scale,
+                  layout, output, max_seq_len, workspace, stream, window, first_tokens, key_exps,
+                  value_exps) -> torch.Tensor:
+    """paged_prefill over a quantised cache and/or with a sliding window."""
+    dev = _one_device(query=query, key_cache=key_cache, value_cache=value_cache,
+                      block_table=block_table, token_to_seq=token_to_seq, positions=positions,
+                      output=output, key_exps=key_exps, value_exps=value_exps,
+                      workspace=workspace)
+    view = _kv_view(key_cache, value_cache, key_exps, value_exps, layout, window, first_tokens)
+    rows = dict(query=query, output=output)
+    dt = _attn_dtype(**rows) if key_exps is not None else _attn_dtype(
+        key_cache=key_cache, value_cache=value_cache, **rows)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous int32 2-D tensor")
+    num_tokens = query.shape[0]
+    for t, n in ((token_to_seq, "token_to_seq"), (positions, "positions")):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{n} must be a contiguous int32 tensor")
+        if t.numel() < num_tokens:
+            raise ValueError("token_to_seq/positions shorter than query")
+    with _on_device(dev):
+        if output is None:
+            # Rows that the kernel leaves unwritten are zeros.
+            output = _stream_empty(tuple(query.shape), dt, dev, stream)
+            with torch.cuda.stream(_as_stream(stream, dev)):
+                output.zero_()
+        if output.shape != query.shape:
+            raise ValueError("output must have the query's shape")
+        p = make_params(key_cache=key_cache, value_cache=value_cache, layout=layout,
+                        num_query_heads=query.shape[1], scale=scale,
+                        num_seqs=block_table.shape[0], max_seq_len=max_seq_len,
+                        max_blocks_per_seq=block_table.shape[1], query=query, output=output,
+                        dtype=dt)
+        if query.shape[2] != p.head_size:
+            raise ValueError(f"query head_size {query.shape[2]} != cache head_size {p.head_size}")
+        nbytes = _lib.load().vaa_paged_attention_prefill_view_workspace_size(
+            ctypes.byref(p), ctypes.byref(view), num_tokens)
+        ws = workspace if workspace is not None else _stream_scratch(nbytes, dev, stream)
+        _lib.call("vaa_paged_attention_prefill_view", ctypes.byref(p), ctypes.byref(view),
+                  query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                  block_table.data_ptr(), token_to_seq.data_ptr(), positions.data_ptr(),
+                  output.data_ptr(), num_tokens, _ptr(ws),
+                  ws.numel() * ws.element_size() if ws is not None else 0,
+                  _lib.stream_handle(stream))
+    return output
 
 
 # ----------------------------------------------------------------- layer ops
