@@ -36,6 +36,13 @@ namespace {
   X(vaa_attention_no_cache_workspace_size)
 #define VAA_DECL(f) decltype(&::f) p_##f = nullptr;
 VAA_FUNCS(VAA_DECL)
+// Entry points over a vaa_kv_view; a library without them leaves these calls to the
+// wrappers.
+#define VAA_VIEW_FUNCS(X)                                                                 \
+  X(vaa_kv_write_slots_q8) X(vaa_kv_read_slots_q8) X(vaa_paged_attention_decode_view)     \
+  X(vaa_paged_attention_decode_view_workspace_size) X(vaa_paged_attention_prefill_view)   \
+  X(vaa_paged_attention_prefill_view_workspace_size)
+VAA_VIEW_FUNCS(VAA_DECL)
 #undef VAA_DECL
 
 using at::Tensor;
@@ -640,6 +647,127 @@ PyObject* no_cache(const Args& a) {
                     a.s(12)));
 }
 
+// ------------------------------------- quantised caches, sliding windows --
+
+// The view of a cache whose fields p already has; ke and ve are both given or both
+// null.  False: fall back.
+bool view_of(const Tensor& kc, const Tensor& vc, const Tensor* ke, const Tensor* ve, bool vllm,
+             int64_t window, int64_t first, int dt, vaa_kv_view* v) {
+  if (!small(window) || !small(first)) return false;
+  v->window = window;
+  v->first_tokens = first;
+  if (!ke || !ve) {
+    v->cache_type = VAA_CACHE_16BIT;
+    return !ke && !ve && dt16(kc) == dt && dt16(vc) == dt;
+  }
+  const int h = vllm ? 2 : 1, t = vllm ? 1 : 2;
+  for (const Tensor* c : {&kc, &vc})
+    if (!on_gpu(*c) || c->scalar_type() != at::kFloat8_e4m3fn) return false;
+  for (const Tensor* e : {ke, ve})
+    if (!on_gpu(*e) || e->scalar_type() != at::kByte || e->dim() != 3 ||
+        e->sizes() != kc.sizes().slice(0, 3))
+      return false;
+  v->cache_type = VAA_CACHE_E4M3;
+  v->key_exps = static_cast<uint8_t*>(ptr(*ke));
+  v->value_exps = static_cast<uint8_t*>(ptr(*ve));
+  v->ke_stride_block = ke->stride(0);
+  v->ke_stride_head = ke->stride(h);
+  v->ke_stride_token = ke->stride(t);
+  v->ve_stride_block = ve->stride(0);
+  v->ve_stride_head = ve->stride(h);
+  v->ve_stride_token = ve->stride(t);
+  return true;
+}
+// Whether the stream's device, the current one, is the tensors'.
+bool current(const Tensor& t, int64_t device) { return t.device().index() == device; }
+
+// (key, value, key_cache, value_cache, key_exps, value_exps, slots, vllm, read, device,
+//  stream)
+PyObject* rows_q8(const Args& a) {
+  const Tensor *k = a.t(0), *v = a.t(1), *kc = a.t(2), *vc = a.t(3), *ke = a.t(4), *ve = a.t(5),
+               *sl = a.t(6);
+  const bool read = a.b(8);
+  if (!k || !v || !kc || !vc || !ke || !ve || !sl || !one_device({k, v, kc, vc, ke, ve, sl}) ||
+      !(read ? p_vaa_kv_read_slots_q8 != nullptr : p_vaa_kv_write_slots_q8 != nullptr) ||
+      !current(*k, a.i(9)))
+    Py_RETURN_FALSE;
+  const int dt = dt16(*k);
+  vaa_attn_params p{};
+  vaa_kv_view view{};
+  int it;
+  if (dt < 0 || dt16(*v) != dt || k->dim() != 3 || !small(k->size(0)) ||
+      !cache4(*kc, *vc, a.b(7), &p) || !view_of(*kc, *vc, ke, ve, a.b(7), 0, 0, dt, &view) ||
+      !write_params(*k, *v, *sl, k->size(0), &p, &it))
+    Py_RETURN_FALSE;
+  p.dtype = dt;
+  auto *kp = static_cast<uint8_t*>(ptr(*kc)), *vp = static_cast<uint8_t*>(ptr(*vc));
+  if (read)
+    return yes(launch(p_vaa_kv_read_slots_q8, &p, &view, kp, vp, ptr(*sl), it, p16(*k), p16(*v),
+                      k->size(0), a.s(10)));
+  return yes(launch(p_vaa_kv_write_slots_q8, &p, &view, kp, vp, ptr(*sl), it, p16(*k), p16(*v),
+                    k->size(0), a.s(10)));
+}
+
+// (query, key_cache, value_cache, key_exps or None, value_exps or None, block_table,
+//  seq_lens, output, vllm, scale, max_seq_len, partition_size, window, first_tokens,
+//  workspace or None, device, stream)
+PyObject* decode_view(const Args& a) {
+  const Tensor *q = a.t(0), *kc = a.t(1), *vc = a.t(2), *ke = a.t(3), *ve = a.t(4), *bt = a.t(5),
+               *sl = a.t(6), *o = a.t(7), *ws = a.t(14);
+  if (!q || !kc || !vc || !none_or_ten(a.a[3]) || !none_or_ten(a.a[4]) || !bt || !sl || !o ||
+      !none_or_ten(a.a[14]) || !one_device({q, kc, vc, ke, ve, bt, sl, o}) ||
+      !p_vaa_paged_attention_decode_view || !p_vaa_paged_attention_decode_view_workspace_size ||
+      !current(*q, a.i(15)))
+    Py_RETURN_FALSE;
+  const int dt = dt16(*q);
+  const bool vllm = a.b(8);
+  vaa_attn_params p{};
+  vaa_kv_view view{};
+  if (dt < 0 || dt16(*o) != dt || !cache4(*kc, *vc, vllm, &p) ||
+      !decode_params(*q, *o, *bt, *sl, sl->numel(), a.f(9), a.i(10), a.i(11), &p) ||
+      o->size(1) != q->size(1) || o->size(2) != q->size(2) ||
+      !view_of(*kc, *vc, ke, ve, vllm, a.i(12), a.i(13), dt, &view))
+    Py_RETURN_FALSE;
+  p.dtype = dt;
+  const size_t need = p_vaa_paged_attention_decode_view_workspace_size(&p, &view, nullptr);
+  if (need && !room(ws, need, *q)) return PyLong_FromSize_t(need);
+  return yes(launch(p_vaa_paged_attention_decode_view, &p, &view, p16(*q), ptr(*kc), ptr(*vc),
+                    static_cast<int32_t*>(ptr(*bt)), static_cast<int32_t*>(ptr(*sl)), p16(*o),
+                    need ? ptr(*ws) : nullptr, need ? ws->nbytes() : 0, a.s(16)));
+}
+
+// (query, key_cache, value_cache, key_exps or None, value_exps or None, block_table,
+//  token_to_seq, positions, output, vllm, scale, max_seq_len, window, first_tokens,
+//  workspace or None, device, stream)
+PyObject* prefill_view(const Args& a) {
+  const Tensor *q = a.t(0), *kc = a.t(1), *vc = a.t(2), *ke = a.t(3), *ve = a.t(4), *bt = a.t(5),
+               *tok = a.t(6), *pos = a.t(7), *o = a.t(8), *ws = a.t(14);
+  if (!q || !kc || !vc || !none_or_ten(a.a[3]) || !none_or_ten(a.a[4]) || !bt || !tok || !pos ||
+      !o || !none_or_ten(a.a[14]) || !one_device({q, kc, vc, ke, ve, bt, tok, pos, o}) ||
+      !p_vaa_paged_attention_prefill_view || !p_vaa_paged_attention_prefill_view_workspace_size ||
+      !current(*q, a.i(15)))
+    Py_RETURN_FALSE;
+  const int dt = dt16(*q);
+  const bool vllm = a.b(9);
+  const int64_t max_len = a.i(11);
+  vaa_attn_params p{};
+  vaa_kv_view view{};
+  if (dt < 0 || dt16(*o) != dt || q->dim() != 3 || o->sizes() != q->sizes() ||
+      !cache4(*kc, *vc, vllm, &p) || !prefill_params(*q, *o, *bt, q->size(0), a.f(10), &p) ||
+      !is_i32(*tok) || !is_i32(*pos) || tok->numel() < q->size(0) || pos->numel() < q->size(0) ||
+      !small(max_len) || !view_of(*kc, *vc, ke, ve, vllm, a.i(12), a.i(13), dt, &view))
+    Py_RETURN_FALSE;
+  p.dtype = dt;
+  p.max_seq_len = max_len;
+  const int n = static_cast<int>(q->size(0));
+  const size_t need = p_vaa_paged_attention_prefill_view_workspace_size(&p, &view, n);
+  if (need && !room(ws, need, *q)) return PyLong_FromSize_t(need);
+  return yes(launch(p_vaa_paged_attention_prefill_view, &p, &view, p16(*q), ptr(*kc), ptr(*vc),
+                    static_cast<int32_t*>(ptr(*bt)), static_cast<int32_t*>(ptr(*tok)),
+                    static_cast<int32_t*>(ptr(*pos)), p16(*o), n, need ? ptr(*ws) : nullptr,
+                    need ? ws->nbytes() : 0, a.s(16)));
+}
+
 // bind(handle): the entry points of the library that _lib.py loaded.
 PyObject* bind(PyObject*, PyObject* arg) {
   void* h = PyLong_AsVoidPtr(arg);
@@ -660,6 +788,9 @@ PyObject* bind(PyObject*, PyObject* arg) {
   }
   VAA_FUNCS(VAA_BIND)
 #undef VAA_BIND
+#define VAA_BIND(f) p_##f = reinterpret_cast<decltype(p_##f)>(dlsym(h, #f));
+  VAA_VIEW_FUNCS(VAA_BIND)
+#undef VAA_BIND
   Py_RETURN_NONE;
 }
 
@@ -678,6 +809,9 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          VAA_METHOD(step_prefill, 16),
                          VAA_METHOD(prefill, 14),
                          VAA_METHOD(no_cache, 13),
+                         VAA_METHOD(rows_q8, 11),
+                         VAA_METHOD(decode_view, 17),
+                         VAA_METHOD(prefill_view, 17),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,
                       nullptr,               nullptr, nullptr, nullptr};

@@ -49,7 +49,11 @@ inline int check_view(const char* what, const vaa_attn_params* p, const vaa_kv_v
     for (int64_t s : exps)
       if (s < 0) return fail(VAA_ERR_INVALID_ARG, "%s: negative exponent stride", what);
   }
-  // Offsets of a tile's lanes are 32-bit bytes.
+  // Offsets inside a block are 32-bit bytes.
+  if (p->k_stride_block >= (int64_t{1} << 31) || p->v_stride_block >= (int64_t{1} << 31) ||
+      p->k_stride_token * p->block_size >= (int64_t{1} << 31) ||
+      p->v_stride_token * p->block_size >= (int64_t{1} << 31))
+    return fail(VAA_ERR_UNSUPPORTED, "%s: a cache block of 2^31 values or more", what);
   if (p->k_stride_token >= (int64_t{1} << 24) || p->v_stride_token >= (int64_t{1} << 24))
     return fail(VAA_ERR_INVALID_ARG, "%s: token stride too large", what);
   return VAA_OK;

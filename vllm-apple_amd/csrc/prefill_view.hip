@@ -61,10 +61,14 @@ struct Args {
   float scale_log2;
   int hd, num_tokens, num_seqs, max_blocks, block_size, kvh, H, G;
   int window, first, n_splits;
+  int bs_shift;  // log2(block_size) where it is a power of two, else -1
   int tiles_x, padded;  // query tiles; workgroups in use (a multiple of 8)
-  int64_t num_blocks;
-  int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;        // bytes
-  int64_t ke_sb, ke_sh, ke_st, ve_sb, ve_sh, ve_st;  // bytes
+  uint32_t num_blocks;  // at most 2^31: block ids are 32-bit
+  // Bytes.  Block and token strides are below 2^32 and 2^25, so that a row's offset
+  // takes 32-bit factors.
+  uint32_t k_sb, k_st, v_sb, v_st;
+  int64_t k_sh, v_sh;
+  int64_t ke_sb, ke_sh, ke_st, ve_sb, ve_sh, ve_st;
   int64_t q_st, q_sh, o_st, o_sh;                    // elements
 };
 
@@ -117,6 +121,11 @@ struct Range {
   int kv_len, first, lo;
 };
 
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (const __attribute__((address_space(3))) char*)p));
+}
+
 struct Window {
   int base, vals;  // lane i: table entry base + i, or -1
 };
@@ -156,8 +165,8 @@ __device__ __forceinline__ void pieces_init(const Args& a, int wave, int lane, P
       pc.vin |= (cv * 8 < a.hd ? 1u : 0u) << i;
     }
     pc.row[i] = r;
-    pc.k[i] = r * static_cast<uint32_t>(a.k_st) + ck * 16;
-    pc.v[i] = r * static_cast<uint32_t>(a.v_st) + cv * 16;
+    pc.k[i] = r * a.k_st + ck * 16;
+    pc.v[i] = r * a.v_st + cv * 16;
   }
 }
 
@@ -174,28 +183,30 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
   const char* vb = a.vc + kvh * a.v_sh;
   char* kl = reinterpret_cast<char*>(kd) + 1024 * (wave * C::NI);
   char* vl = reinterpret_cast<char*>(vd) + 1024 * (wave * C::NI);
-  const uint32_t ka = __builtin_amdgcn_readfirstlane(
-      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(kl)));
-  const uint32_t va = __builtin_amdgcn_readfirstlane(
-      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(vl)));
-  uint32_t ok = low16(rg.kv_len - k0) & (~low16(rg.lo - k0) | low16(rg.first - k0));
-  const int bi = k0 / a.block_size;
+  const uint32_t ka = __builtin_amdgcn_readfirstlane(lds_address(kl));
+  const uint32_t va = __builtin_amdgcn_readfirstlane(lds_address(vl));
+  // The rows that are read; all of them but at the ends of what is seen.
+  uint32_t ok = 0xFFFFu;
+  if (k0 + 16 > rg.kv_len || (k0 < rg.lo && k0 + 16 > rg.first))
+    ok = low16(rg.kv_len - k0) & (~low16(rg.lo - k0) | low16(rg.first - k0));
+  const bool any_block = kAny && a.block_size % 16 != 0;
+  const int bi = a.bs_shift >= 0 ? k0 >> a.bs_shift : k0 / a.block_size;
   if (ok) {
-    const int last = min(k0 + 15, rg.kv_len - 1) / a.block_size;
+    const int last = any_block ? min(k0 + 15, rg.kv_len - 1) / a.block_size : bi;
     if (bi < w.base || last >= w.base + kWave) {
       w.base = bi;
       const int e = bi + lane;
       w.vals = e < a.max_blocks ? bts[e] : -1;
     }
   }
-  if (kAny && a.block_size % 16 != 0) {
+  if (any_block) {
     // Rows that find their own blocks.
     auto row_at = [&](int r, int64_t& p, int& rin) {
       const int tok = k0 + r, b = tok / a.block_size;
       const int e = __shfl(w.vals, max(0, min(kWave - 1, b - w.base)), kWave);
       p = e;
       rin = tok - b * a.block_size;
-      return ((ok >> r) & 1u) && e >= 0 && e < a.num_blocks;
+      return ((ok >> r) & 1u) && static_cast<uint32_t>(e) < a.num_blocks;
     };
     int64_t p;
     int rin;
@@ -205,8 +216,8 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
       const int r = pc.row[i];
       const bool good = row_at(r, p, rin);
       // pc's offsets hold r rows; the row's own block replaces them.
-      const char* ks = kb + p * a.k_sb + rin * a.k_st + (pc.k[i] - r * (uint32_t)a.k_st);
-      const char* vs = vb + p * a.v_sb + rin * a.v_st + (pc.v[i] - r * (uint32_t)a.v_st);
+      const char* ks = kb + p * a.k_sb + rin * a.k_st + (pc.k[i] - r * a.k_st);
+      const char* vs = vb + p * a.v_sb + rin * a.v_st + (pc.v[i] - r * a.v_st);
       const bool kin = good && ((pc.kin >> i) & 1u), vin = good && ((pc.vin >> i) & 1u);
       if constexpr (Q8) {
         gr.k[i] = kin ? ld16(ks) : z;
@@ -224,22 +235,22 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
     return;
   }
   // The group lies in one block.
-  int64_t phys = 0;
+  uint32_t phys = 0;
   if (ok) {
-    phys = __builtin_amdgcn_readlane(w.vals, bi - w.base);
-    if (phys < 0 || phys >= a.num_blocks) {
+    phys = static_cast<uint32_t>(__builtin_amdgcn_readlane(w.vals, bi - w.base));
+    if (phys >= a.num_blocks) {
       ok = 0;
       phys = 0;
     }
   }
-  const int rin = k0 - bi * a.block_size;
-  kb += phys * a.k_sb + rin * a.k_st;
-  vb += phys * a.v_sb + rin * a.v_st;
+  const uint32_t rin = k0 - bi * a.block_size;
+  kb += static_cast<uint64_t>(phys) * a.k_sb + rin * a.k_st;
+  vb += static_cast<uint64_t>(phys) * a.v_sb + rin * a.v_st;
   gr.ok = ok;
   if constexpr (Q8) {
     const uint8_t* ke = a.ke + phys * a.ke_sb + kvh * a.ke_sh + rin * a.ke_st;
     const uint8_t* ve = a.ve + phys * a.ve_sb + kvh * a.ve_sh + rin * a.ve_st;
-    const bool whole = ok == 0xFFFFu && !kAny && 16 * C::GCH % kWave == 0;
+    constexpr bool kFull = !kAny && 16 * C::GCH % kWave == 0;  // every lane's pieces lie in the rows
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
       const bool good = (ok >> pc.row[i]) & 1u;
@@ -247,7 +258,7 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
       gr.v[i] = z;
       gr.ke[i] = 0;
       gr.ve[i] = 0;
-      if (whole || (good && ((pc.kin >> i) & 1u))) {
+      if (good && (kFull || ((pc.kin >> i) & 1u))) {
         gr.k[i] = ld16(kb + pc.k[i]);
         gr.v[i] = ld16(vb + pc.v[i]);
         gr.ke[i] = ke[pc.row[i] * a.ke_st];
@@ -266,9 +277,9 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
       const bool good = (ok >> pc.row[i]) & 1u;
-      if (good && ((pc.kin >> i) & 1u)) dma16(kb + pc.k[i], ka + 1024 * i);
+      if (good && (!kAny || ((pc.kin >> i) & 1u))) dma16(kb + pc.k[i], ka + 1024 * i);
       else *reinterpret_cast<u32x4*>(kl + 1024 * i + 16 * lane) = z;
-      if (good && ((pc.vin >> i) & 1u)) dma16(vb + pc.v[i], va + 1024 * i);
+      if (good && (!kAny || ((pc.vin >> i) & 1u))) dma16(vb + pc.v[i], va + 1024 * i);
       else *reinterpret_cast<u32x4*>(vl + 1024 * i + 16 * lane) = z;
     }
   }
@@ -310,10 +321,16 @@ __device__ __forceinline__ void deliver(const Group<D, Q8>& gr, const Pieces<D, 
   if (lane == 0) reinterpret_cast<uint16_t*>(&sh.ok[buf])[wave] = static_cast<uint16_t>(gr.ok);
 }
 
-// Per-lane LDS addresses of the MFMA operands.
+// Per-lane LDS addresses of the MFMA operands: K's for step s, V's for dim tile dt.
+// The rows are a power of two wide but for D = 96, and the chunk swizzle is an XOR,
+// so the address of a later step is the first one's XOR a constant: one register
+// instead of one per step (the accumulators leave few).
 template <int D>
 struct Lanes {
-  int k[D / 16], v[D / 32];
+  static constexpr bool XOR = D != 96;
+  int k[XOR ? 1 : D / 16], v[XOR ? 1 : D / 32];
+  __device__ __forceinline__ int kaddr(int s) const { return XOR ? k[0] ^ (16 * s) : k[s]; }
+  __device__ __forceinline__ int vaddr(int dt) const { return XOR ? v[0] ^ (64 * dt) : v[dt]; }
 };
 
 // A row's state: its running maximum (log2 domain), its part of the sum, O^T.
@@ -327,7 +344,7 @@ struct State {
 // What a row sees of the sequence: keys up to lim, from lo on or below first.  A row
 // that is never written sees everything, so that it asks for no mask.
 struct Sees {
-  int lim, lo, first;
+  int lim, lo;
 };
 
 constexpr int kAheadK = 4, kAheadV = 4;  // LDS operand reads ahead of their MFMAs
@@ -339,31 +356,34 @@ constexpr int kAheadK = 4, kAheadV = 4;  // LDS operand reads ahead of their MFM
 template <int D, typename T, bool Q8, bool kCareful>
 __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f16* vt, int key0,
                                           const Sees& see, const Shared& sh, int buf, int hb,
-                                          const Lanes<D>& L, const u32x4 (&qb)[D / 16],
+                                          Lanes<D> L, const u32x4 (&qb)[D / 16],
                                           State<D>& st) {
   using C = Cfg<D, Q8>;
+  // The XORs stay in the loop.
+  if constexpr (Lanes<D>::XOR) asm volatile("" : "+v"(L.k[0]), "+v"(L.v[0]));
   using PT = typename std::conditional<Q8, f16, T>::type;  // type of V and P
   using X4 = typename Elem<PT>::x4;
   using P8 = typename Elem<PT>::x8;
   using X8 = typename Elem<T>::x8;
   constexpr bool kPair = !Q8 && Elem<T>::kSplitP;
-  // Whether some row of the wave sees less than the whole tile, and then the keys
-  // that this row sees.
-  uint64_t seen = sh.ok[buf];
-  const bool masked =
-      __builtin_amdgcn_ballot_w64(seen != ~0ull || see.lim - key0 < kKT - 1 ||
-                                  (see.lo > key0 && see.first - key0 < kKT)) != 0;
-  if (masked) {
-    seen &= low64(see.lim + 1 - key0) & (~low64(see.lo - key0) | low64(see.first - key0));
-    if (__builtin_amdgcn_ballot_w64(seen != 0) == 0) return;  // nothing for this wave
+  // By position, does every row of the wave see the whole tile, or none of it any?
+  uint64_t seen = ~0ull;
+  const bool inside = see.lim - key0 >= kKT - 1 && (see.lo <= key0 || a.first - key0 >= kKT);
+  const bool whole = __builtin_amdgcn_ballot_w64(inside) == ~0ull;
+  if (!whole) {
+    seen = low64(see.lim + 1 - key0) & (~low64(see.lo - key0) | low64(a.first - key0));
+    if (__builtin_amdgcn_ballot_w64(seen != 0) == 0) return;
   }
+  // What the tile holds, and its exponents: used behind the first product.
+  const uint64_t held = sh.ok[buf];
+  const uint32_t held_e = Q8 ? sh.ev[buf] : 0;
 
   const char* kbytes = reinterpret_cast<const char*>(kt);
   const char* vbytes = reinterpret_cast<const char*>(vt);
   constexpr int NKR = 2 * C::NK, NPV = C::NDT * 4;
   u32x4 kA[NKR];
   auto kread = [&](int i) {
-    kA[i] = *reinterpret_cast<const u32x4*>(kbytes + L.k[i >> 1] + 32 * (i & 1) * C::ROWB);
+    kA[i] = *reinterpret_cast<const u32x4*>(kbytes + L.kaddr(i >> 1) + 32 * (i & 1) * C::ROWB);
   };
 #pragma unroll
   for (int i = 0; i < kAheadK && i < NKR; ++i) kread(i);
@@ -383,7 +403,7 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
   X4 vlo[NPV], vhi[NPV];
   auto vread = [&](int i) {
     const int g = i / C::NDT, dt = i % C::NDT;
-    const f16* vp = reinterpret_cast<const f16*>(vbytes + L.v[dt] + 16 * g * C::ROWB);
+    const f16* vp = reinterpret_cast<const f16*>(vbytes + L.vaddr(dt) + 16 * g * C::ROWB);
     vlo[i] = lds_tr4<PT>(vp);
     vhi[i] = lds_tr4<PT>(vp + 8 * D);
   };
@@ -391,7 +411,8 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
   for (int i = 0; i < kAheadV && i < NPV; ++i) vread(i);
   __builtin_amdgcn_sched_barrier(0);
   // Lane holds keys 32j + 8(r/4) + 4hb + r%4 of its row.
-  if (masked) {
+  seen &= held;
+  if (!whole || __builtin_amdgcn_ballot_w64(held == ~0ull) != ~0ull) {
     const uint64_t mine = seen >> (4 * hb);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -415,13 +436,10 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
     st.m = mx;
   }
   const float sub = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[j][r] = fast_exp2(fmaf(s[j][r], a.scale_log2, -sub));
   bool even = true;  // the groups' V share the exponent that acc is relative to
+  uint32_t ev = 0;
   if constexpr (Q8) {
-    const uint32_t ev = __builtin_amdgcn_readfirstlane(static_cast<int>(sh.ev[buf]));
+    ev = __builtin_amdgcn_readfirstlane(static_cast<int>(held_e));
     const int top = max(max(ev >> 24, (ev >> 16) & 255), max((ev >> 8) & 255, ev & 255));
     if (top > st.e) {
       const float alpha = __uint_as_float(static_cast<uint32_t>(max(1, 127 + st.e - top)) << 23);
@@ -430,29 +448,45 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
       st.e = top;
     }
     even = ev == static_cast<uint32_t>(st.e) * 0x01010101u;
-    if (!even) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int eg = (ev >> (8 * (2 * j + (r >> 3)))) & 255;
-          st.l += s[j][r];
-          s[j][r] *= __uint_as_float(static_cast<uint32_t>(max(1, 127 + eg - st.e)) << 23);
-        }
-    }
   }
   P8 pb[4], pl[4];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int g = 2 * j + (r >> 3);
-      pb[g][r & 7] = Elem<PT>::from_f(s[j][r]);
-      if constexpr (kPair) {
-        pl[g][r & 7] = Elem<PT>::from_f(s[j][r] - Elem<PT>::to_f(pb[g][r & 7]));
-        st.l += s[j][r];
-      }
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef decltype(Elem<PT>::from_f(0.f)) E2 __attribute__((ext_vector_type(2)));
+  // P of the group's values r, r + 1, to its pair of 16-bit values.
+  auto put = [&](int g, int i, f32x2 p) {
+    const E2 h = __builtin_convertvector(p, E2);
+    pb[g][i] = h[0];
+    pb[g][i + 1] = h[1];
+    if constexpr (kPair) {
+      const f32x2 back = {Elem<PT>::to_f(h[0]), Elem<PT>::to_f(h[1])};
+      const E2 l = __builtin_convertvector(f32x2{p[0] - back[0], p[1] - back[1]}, E2);
+      pl[g][i] = l[0];
+      pl[g][i + 1] = l[1];
+      st.l += p[0] + p[1];
     }
+  };
+  if (even) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2)
+        put(2 * j + (r >> 3), r & 7,
+            f32x2{fast_exp2(fmaf(s[j][r], a.scale_log2, -sub)),
+                  fast_exp2(fmaf(s[j][r + 1], a.scale_log2, -sub))});
+  } else {
+    // A tile that raises E: the sum takes P itself, the product P 2^(E_g - E).
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const int eg = (ev >> (8 * (2 * j + (r >> 3)))) & 255;
+        const float w = __uint_as_float(static_cast<uint32_t>(max(1, 127 + eg - st.e)) << 23);
+        const f32x2 p = {fast_exp2(fmaf(s[j][r], a.scale_log2, -sub)),
+                         fast_exp2(fmaf(s[j][r + 1], a.scale_log2, -sub))};
+        st.l += p[0] + p[1];
+        put(2 * j + (r >> 3), r & 7, f32x2{p[0] * w, p[1] * w});
+      }
+  }
   if constexpr (!kPair) {
     // The sum takes P as the product sees it, two values per v_dot2_f32_f16.
     if (even) {
@@ -522,7 +556,7 @@ __device__ __forceinline__ bool row_place(const Args& a, int64_t tok, int& seq, 
 
 // All keys of this workgroup's split for its rows, sequence by sequence.
 template <int D, typename T, bool Q8, bool kAny, bool kCareful>
-__device__ __forceinline__ void walk(const Args& a, f16* k0s, f16* k1s, f16* v0s, f16* v1s,
+__device__ __forceinline__ void walk(const Args& a, f16* ks, f16* vs,
                                      Shared& sh, int kvh, int split, int wave, int lane,
                                      bool row_ok, int tseq, int tpos, const Lanes<D>& L,
                                      const Pieces<D, Q8>& pc, const u32x4 (&qb)[D / 16],
@@ -547,6 +581,7 @@ __device__ __forceinline__ void walk(const Args& a, f16* k0s, f16* k1s, f16* v0s
     s = sh.red[0][0];
 #pragma unroll
     for (int w = 1; w < kWavesV; ++w) s = min(s, sh.red[0][w]);
+    s = __builtin_amdgcn_readfirstlane(s);
     if (s == INT32_MAX) break;
     const bool active = !done && tseq == s;
     int pmax = wave_max_i(active ? tpos : -1), pmin = wave_min_i(active ? tpos : INT32_MAX);
@@ -565,11 +600,10 @@ __device__ __forceinline__ void walk(const Args& a, f16* k0s, f16* k1s, f16* v0s
     pmax = __builtin_amdgcn_readfirstlane(pmax);
     pmin = __builtin_amdgcn_readfirstlane(pmin);
     const int32_t* bts = a.bt + static_cast<int64_t>(s) * a.max_blocks;
-    Sees see{row_ok ? -1 : INT32_MAX - 1, 0, 0};
+    Sees see{row_ok ? -1 : INT32_MAX - 1, 0};
     if (active) {
       see.lim = tpos;
       see.lo = a.window > 0 ? max(0, tpos + 1 - a.window) : 0;
-      see.first = a.first;
     }
     Range rg;
     rg.kv_len = pmax + 1;
@@ -584,14 +618,16 @@ __device__ __forceinline__ void walk(const Args& a, f16* k0s, f16* k1s, f16* v0s
       auto key_of = [&](int t) { return (t < nf ? t : t + skip) * kKT; };
       Window w{-(1 << 30), -1};
       Group<D, Q8> gr;
-      auto get = [&](int t, f16* kd, f16* vd) {
+      auto get = [&](int t, int buf) {
         if (t < t_hi)
-          fetch<D, Q8, kAny>(a, bts, kvh, key_of(t) + 16 * wave, rg, wave, lane, pc, w, kd, vd,
-                             gr);
+          fetch<D, Q8, kAny>(a, bts, kvh, key_of(t) + 16 * wave, rg, wave, lane, pc, w,
+                             ks + buf * C::TILE, vs + buf * C::TILE, gr);
       };
       // The tile is in LDS: codes converted, direct loads landed, for every wave.
-      auto put = [&](int t, f16* kd, f16* vd, int buf) {
-        if (t < t_hi) deliver<D, T, Q8>(gr, pc, wave, lane, kd, vd, sh, buf, e_run);
+      auto put = [&](int t, int buf) {
+        if (t < t_hi)
+          deliver<D, T, Q8>(gr, pc, wave, lane, ks + buf * C::TILE, vs + buf * C::TILE, sh, buf,
+                            e_run);
         wait_all();
         __builtin_amdgcn_s_barrier();
         if (Q8 && t < t_hi) {
@@ -600,16 +636,13 @@ __device__ __forceinline__ void walk(const Args& a, f16* k0s, f16* k1s, f16* v0s
                                                   max((ev >> 8) & 255, ev & 255))));
         }
       };
-      get(t_lo, k0s, v0s);
-      put(t_lo, k0s, v0s, 0);
-      for (int t = t_lo; t < t_hi; t += 2) {
-        get(t + 1, k1s, v1s);
-        tile_math<D, T, Q8, kCareful>(a, k0s, v0s, key_of(t), see, sh, 0, hb, L, qb, st);
-        put(t + 1, k1s, v1s, 1);
-        if (t + 1 >= t_hi) break;
-        get(t + 2, k0s, v0s);
-        tile_math<D, T, Q8, kCareful>(a, k1s, v1s, key_of(t + 1), see, sh, 1, hb, L, qb, st);
-        put(t + 2, k0s, v0s, 0);
+      get(t_lo, 0);
+      put(t_lo, 0);
+      for (int t = t_lo, buf = 0; t < t_hi; ++t, buf ^= 1) {
+        get(t + 1, buf ^ 1);
+        tile_math<D, T, Q8, kCareful>(a, ks + buf * C::TILE, vs + buf * C::TILE, key_of(t), see, sh,
+                                      buf, hb, L, qb, st);
+        put(t + 1, buf ^ 1);
       }
     }
     done = done || active;
@@ -620,10 +653,8 @@ template <int D, typename T, bool Q8, bool kAny>
 __global__ void __launch_bounds__(kThreadsV) __attribute__((amdgpu_waves_per_eu(2, 2)))
 prefill_view_kernel(Args a) {
   using C = Cfg<D, Q8>;
-  __shared__ __align__(16) f16 k0s[C::TILE];
-  __shared__ __align__(16) f16 k1s[C::TILE];
-  __shared__ __align__(16) f16 v0s[C::TILE];
-  __shared__ __align__(16) f16 v1s[C::TILE];
+  __shared__ __align__(16) f16 ks[2 * C::TILE];
+  __shared__ __align__(16) f16 vs[2 * C::TILE];
   __shared__ Shared sh;
 
   // Consecutive workgroup ids go to the 8 XCDs in turn; each XCD gets a contiguous
@@ -658,20 +689,20 @@ prefill_view_kernel(Args a) {
   }
   Lanes<D> L;
 #pragma unroll
-  for (int s = 0; s < C::NK; ++s)
+  for (int s = 0; s < (Lanes<D>::XOR ? 1 : C::NK); ++s)
     L.k[s] = qj * C::ROWB + ((hb * (C::CH / 2) + s) ^ swzk<D>(qj)) * 16;
   {
     const int g16 = lane >> 4, i16 = lane & 15;
     const int r = 4 * hb + (i16 >> 2), j4 = i16 & 3;
 #pragma unroll
-    for (int dt = 0; dt < C::NDT; ++dt)
+    for (int dt = 0; dt < (Lanes<D>::XOR ? 1 : C::NDT); ++dt)
       L.v[dt] = r * C::ROWB + ((4 * dt + 2 * (g16 & 1) + (j4 >> 1)) ^ swz<D>(r)) * 16 +
                 (j4 & 1) * 8;
   }
   Pieces<D, Q8> pc;
   pieces_init<D, Q8>(a, wave, lane, pc);
   State<D> st;
-  walk<D, T, Q8, kAny, false>(a, k0s, k1s, v0s, v1s, sh, kvh, split, wave, lane, row_ok, tseq,
+  walk<D, T, Q8, kAny, false>(a, ks, vs, sh, kvh, split, wave, lane, row_ok, tseq,
                               tpos, L, pc, qb, st);
   {
     // An infinity or a NaN in O^T: all over again with care, since it may come from a
@@ -688,7 +719,7 @@ prefill_view_kernel(Args a) {
 #pragma unroll
     for (int w = 0; w < kWavesV; ++w) any |= sh.bad[w];
     if (__builtin_amdgcn_readfirstlane(any)) {
-      walk<D, T, Q8, kAny, true>(a, k0s, k1s, v0s, v1s, sh, kvh, split, wave, lane, row_ok, tseq,
+      walk<D, T, Q8, kAny, true>(a, ks, vs, sh, kvh, split, wave, lane, row_ok, tseq,
                                  tpos, L, pc, qb, st);
     }
   }
@@ -901,12 +932,17 @@ extern "C" int vaa_paged_attention_prefill_view(const vaa_attn_params* p, const 
   a.G = p->queries_per_kv;
   a.window = view->window;
   a.first = view->first_tokens;
+  a.bs_shift = (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
   a.tiles_x = static_cast<int>(query_tiles(p, num_tokens));
   a.padded = (a.tiles_x * a.kvh + kXcds - 1) / kXcds * kXcds;
-  a.num_blocks = p->num_blocks;
+  a.num_blocks = static_cast<uint32_t>(std::min<int64_t>(p->num_blocks, int64_t{1} << 31));
   const int w = q8 ? 1 : 2;  // bytes of a cached value
-  a.k_sb = p->k_stride_block * w; a.k_sh = p->k_stride_head * w; a.k_st = p->k_stride_token * w;
-  a.v_sb = p->v_stride_block * w; a.v_sh = p->v_stride_head * w; a.v_st = p->v_stride_token * w;
+  a.k_sb = static_cast<uint32_t>(p->k_stride_block * w);
+  a.v_sb = static_cast<uint32_t>(p->v_stride_block * w);
+  a.k_st = static_cast<uint32_t>(p->k_stride_token * w);
+  a.v_st = static_cast<uint32_t>(p->v_stride_token * w);
+  a.k_sh = p->k_stride_head * w;
+  a.v_sh = p->v_stride_head * w;
   a.ke_sb = view->ke_stride_block; a.ke_sh = view->ke_stride_head;
   a.ke_st = view->ke_stride_token;
   a.ve_sb = view->ve_stride_block; a.ve_sh = view->ve_stride_head;

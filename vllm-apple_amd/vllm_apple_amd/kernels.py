@@ -958,6 +958,11 @@ def _rows_call(name: str, key: torch.Tensor, value: torch.Tensor, key_cache: tor
                value_cache: torch.Tensor, key_exps: torch.Tensor, value_exps: torch.Tensor,
                slot_mapping: torch.Tensor, layout: str, stream) -> None:
     """vaa_kv_write_slots_q8 or vaa_kv_read_slots_q8."""
+    if layout in _IS_VLLM and key.is_cuda and _lib.host().rows_q8(
+            key, value, key_cache, value_cache, key_exps, value_exps, slot_mapping,
+            _IS_VLLM[layout], name == "vaa_kv_read_slots_q8", torch._C._cuda_getDevice(),
+            _lib.stream_handle(stream)) is True:
+        return
     dev = _one_device(key=key, value=value, key_cache=key_cache, value_cache=value_cache,
                       key_exps=key_exps, value_exps=value_exps, slot_mapping=slot_mapping)
     dt = _attn_dtype(key=key, value=value)
@@ -1016,21 +1021,49 @@ def _as_stream(stream, device: torch.device) -> torch.cuda.Stream:
 def _view_partition(seq_lens_host, query: torch.Tensor, num_kv_heads: int, window: int,
                     first_tokens: int, quantised: bool) -> int:
     """The split-K mode of a decode over a view from its host lengths: the choice for
-    the tokens that are seen, two quantised ones counted as one."""
+    the tokens that are seen, two quantised ones counted as one.  Memoised per length
+    tuple, as that is."""
     lens = _int_tuple(seq_lens_host)
+    key = (lens, query.shape[1], num_kv_heads, window, first_tokens, quantised, query.device)
+    hit = _view_partition_cache.get(key)
+    if hit is not None:
+        return hit
     if window:
         top = window + first_tokens
         lens = tuple(min(n, top) for n in lens)
     if quantised:
         lens = tuple((n + 1) // 2 for n in lens)
     part = _decode_partition(query, num_kv_heads, lens, False)
-    return 2 * part if quantised and part > 0 else part
+    if quantised and part > 0:
+        part *= 2
+    if len(_view_partition_cache) > 4096:
+        _view_partition_cache.clear()
+    _view_partition_cache[key] = part
+    return part
+
+
+_view_partition_cache: dict = {}
 
 
 def _decode_view(query, key_cache, value_cache, block_table, seq_lens, *, scale, max_seq_len,
                  layout, output, partition_size, workspace, seq_lens_host, stream, window,
                  first_tokens, key_exps, value_exps) -> torch.Tensor:
     """paged_decode over a quantised cache and/or with a sliding window."""
+    if query.is_cuda and output is not None and layout in _IS_VLLM and key_cache.dim() == 4 \
+            and query.dim() == 3:
+        part, vllm = partition_size, _IS_VLLM[layout]
+        if part == 0 and seq_lens_host is not None:
+            part = _view_partition(seq_lens_host, query, key_cache.shape[2 if vllm else 1], window,
+                                   first_tokens, key_exps is not None)
+        args = (query, key_cache, value_cache, key_exps, value_exps, block_table, seq_lens, output,
+                vllm, scale, max_seq_len, part, window, first_tokens)
+        where, native = (torch._C._cuda_getDevice(), _lib.stream_handle(stream)), \
+            _lib.host().decode_view
+        done = native(*args, workspace, *where)
+        if done is not True and done and workspace is None:
+            done = native(*args, _stream_scratch(done, query.device, stream), *where)
+        if done is True:
+            return output
     dev = _one_device(query=query, key_cache=key_cache, value_cache=value_cache,
                       block_table=block_table, seq_lens=seq_lens, output=output,
                       key_exps=key_exps, value_exps=value_exps, workspace=workspace)
@@ -1073,6 +1106,16 @@ def _prefill_view(query, key_cache, value_cache, block_table, token_to_seq, posi
                   layout, output, max_seq_len, workspace, stream, window, first_tokens, key_exps,
                   value_exps) -> torch.Tensor:
     """paged_prefill over a quantised cache and/or with a sliding window."""
+    if query.is_cuda and output is not None and layout in _IS_VLLM:
+        args = (query, key_cache, value_cache, key_exps, value_exps, block_table, token_to_seq,
+                positions, output, _IS_VLLM[layout], scale, max_seq_len, window, first_tokens)
+        where, native = (torch._C._cuda_getDevice(), _lib.stream_handle(stream)), \
+            _lib.host().prefill_view
+        done = native(*args, workspace, *where)
+        if done is not True and done and workspace is None:
+            done = native(*args, _stream_scratch(done, query.device, stream), *where)
+        if done is True:
+            return output
     dev = _one_device(query=query, key_cache=key_cache, value_cache=value_cache,
                       block_table=block_table, token_to_seq=token_to_seq, positions=positions,
                       output=output, key_exps=key_exps, value_exps=value_exps,
