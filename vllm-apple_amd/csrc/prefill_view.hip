@@ -130,54 +130,40 @@ struct Window {
   int base, vals;  // lane i: table entry base + i, or -1
 };
 
-// This lane's pieces of a 16-key group: row and byte offset inside the group's rows
-// for load i.  16-bit pieces are the ones that the direct load's slot holds.
-template <int D, bool Q8>
-struct Pieces {
-  using C = Cfg<D, Q8>;
-  uint32_t k[C::NI], v[C::NI];
-  int row[C::NI];
-  uint32_t kin, vin;  // bit i: the piece lies below hd (and, Q8, in the group)
-};
+// The lane, computed anew (two instructions) instead of kept in a register: the
+// accumulators leave few, and one that is spilled in the loop waits for the loads.
+__device__ __forceinline__ int lane_now() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
 
+// This lane's piece of a 16-key group for load i: row, and byte offset in the cached
+// row of its K and V chunk.  16-bit pieces are the ones that the direct load's slot
+// holds.
+struct Piece {
+  int row;
+  uint32_t k, v;
+  bool in;  // Q8: the piece lies in the group (D = 96 and 32 leave some over)
+};
 template <int D, bool Q8>
-__device__ __forceinline__ void pieces_init(const Args& a, int wave, int lane, Pieces<D, Q8>& pc) {
+__device__ __forceinline__ Piece piece(int i, int lane) {
   using C = Cfg<D, Q8>;
-  pc.kin = 0;
-  pc.vin = 0;
-#pragma unroll
-  for (int i = 0; i < C::NI; ++i) {
-    int r, ck, cv;
-    if constexpr (Q8) {
-      const int f = i * kWave + lane;
-      r = f / C::GCH;
-      ck = cv = f % C::GCH;
-      const bool in = r < 16 && ck * 16 < a.hd;
-      pc.kin |= (in ? 1u : 0u) << i;
-      pc.vin |= (in ? 1u : 0u) << i;
-      r &= 15;
-    } else {
-      const int f = 64 * (wave * C::NI + i) + lane, R = f / C::CH;
-      r = R & 15;
-      ck = (f % C::CH) ^ swzk<D>(R);
-      cv = (f % C::CH) ^ swz<D>(R);
-      pc.kin |= (ck * 8 < a.hd ? 1u : 0u) << i;
-      pc.vin |= (cv * 8 < a.hd ? 1u : 0u) << i;
-    }
-    pc.row[i] = r;
-    pc.k[i] = r * a.k_st + ck * 16;
-    pc.v[i] = r * a.v_st + cv * 16;
-  }
+  const int f = 64 * i + lane, r = f / C::GCH, c = f % C::GCH;
+  if constexpr (Q8)
+    return {r & 15, 16u * c, 16u * c, r < 16};
+  else
+    return {r, 16u * (c ^ swzk<D>(r)), 16u * (c ^ swz<D>(r)), true};
 }
 
 // Starts the loads of keys k0 .. k0 + 15, this wave's group of a tile.  Rows that no
 // row of the workgroup sees, or in a missing block, become zeros.
 template <int D, bool Q8, bool kAny>
 __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh, int k0,
-                                      const Range& rg, int wave, int lane,
-                                      const Pieces<D, Q8>& pc, Window& w, f16* kd, f16* vd,
+                                      const Range& rg, int wave, Window& w, f16* kd, f16* vd,
                                       Group<D, Q8>& gr) {
   using C = Cfg<D, Q8>;
+  const int lane = lane_now();
   const u32x4 z = {0u, 0u, 0u, 0u};
   const char* kb = a.kc + kvh * a.k_sh;
   const char* vb = a.vc + kvh * a.v_sh;
@@ -199,6 +185,7 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
       w.vals = e < a.max_blocks ? bts[e] : -1;
     }
   }
+  const uint32_t row_bytes = a.hd * (Q8 ? 1 : 2);  // kAny: pieces past them are zeros
   if (any_block) {
     // Rows that find their own blocks.
     auto row_at = [&](int r, int64_t& p, int& rin) {
@@ -213,12 +200,11 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
     ok = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(row_at(lane & 15, p, rin))) & 0xFFFFu;
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
-      const int r = pc.row[i];
-      const bool good = row_at(r, p, rin);
-      // pc's offsets hold r rows; the row's own block replaces them.
-      const char* ks = kb + p * a.k_sb + rin * a.k_st + (pc.k[i] - r * a.k_st);
-      const char* vs = vb + p * a.v_sb + rin * a.v_st + (pc.v[i] - r * a.v_st);
-      const bool kin = good && ((pc.kin >> i) & 1u), vin = good && ((pc.vin >> i) & 1u);
+      const Piece pc = piece<D, Q8>(i, lane);
+      const bool good = row_at(pc.row, p, rin) && pc.in;
+      const char* ks = kb + p * a.k_sb + rin * a.k_st + pc.k;
+      const char* vs = vb + p * a.v_sb + rin * a.v_st + pc.v;
+      const bool kin = good && pc.k < row_bytes, vin = good && pc.v < row_bytes;
       if constexpr (Q8) {
         gr.k[i] = kin ? ld16(ks) : z;
         gr.v[i] = vin ? ld16(vs) : z;
@@ -253,44 +239,53 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
     constexpr bool kFull = !kAny && 16 * C::GCH % kWave == 0;  // every lane's pieces lie in the rows
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
-      const bool good = (ok >> pc.row[i]) & 1u;
+      const Piece pc = piece<D, Q8>(i, lane);
+      const bool good = ((ok >> pc.row) & 1u) && pc.in;
       gr.k[i] = z;
       gr.v[i] = z;
       gr.ke[i] = 0;
       gr.ve[i] = 0;
-      if (good && (kFull || ((pc.kin >> i) & 1u))) {
-        gr.k[i] = ld16(kb + pc.k[i]);
-        gr.v[i] = ld16(vb + pc.v[i]);
-        gr.ke[i] = ke[pc.row[i] * a.ke_st];
-        gr.ve[i] = ve[pc.row[i] * a.ve_st];
+      if (good && (kFull || pc.k < row_bytes)) {
+        gr.k[i] = ld16(kb + pc.row * a.k_st + pc.k);
+        gr.v[i] = ld16(vb + pc.row * a.v_st + pc.v);
+      }
+      if (good) {
+        gr.ke[i] = ke[pc.row * a.ke_st];
+        gr.ve[i] = ve[pc.row * a.ve_st];
       }
     }
   } else {
     if (!kAny && ok == 0xFFFFu) {
 #pragma unroll
       for (int i = 0; i < C::NI; ++i) {
-        dma16s(kb, pc.k[i], ka + 1024 * i);
-        dma16s(vb, pc.v[i], va + 1024 * i);
+        const Piece pc = piece<D, Q8>(i, lane);
+        dma16s(kb, pc.row * a.k_st + pc.k, ka + 1024 * i);
+        dma16s(vb, pc.row * a.v_st + pc.v, va + 1024 * i);
       }
       return;
     }
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
-      const bool good = (ok >> pc.row[i]) & 1u;
-      if (good && (!kAny || ((pc.kin >> i) & 1u))) dma16(kb + pc.k[i], ka + 1024 * i);
-      else *reinterpret_cast<u32x4*>(kl + 1024 * i + 16 * lane) = z;
-      if (good && (!kAny || ((pc.vin >> i) & 1u))) dma16(vb + pc.v[i], va + 1024 * i);
-      else *reinterpret_cast<u32x4*>(vl + 1024 * i + 16 * lane) = z;
+      const Piece pc = piece<D, Q8>(i, lane);
+      const bool good = (ok >> pc.row) & 1u;
+      if (good && (!kAny || pc.k < row_bytes))
+        dma16(kb + pc.row * a.k_st + pc.k, ka + 1024 * i);
+      else
+        *reinterpret_cast<u32x4*>(kl + 1024 * i + 16 * lane) = z;
+      if (good && (!kAny || pc.v < row_bytes))
+        dma16(vb + pc.row * a.v_st + pc.v, va + 1024 * i);
+      else
+        *reinterpret_cast<u32x4*>(vl + 1024 * i + 16 * lane) = z;
     }
   }
 }
 
 // Q8: the group's codes as 16-bit values in LDS.  Either way its rows in sh.
 template <int D, typename T, bool Q8>
-__device__ __forceinline__ void deliver(const Group<D, Q8>& gr, const Pieces<D, Q8>& pc, int wave,
-                                        int lane, f16* kd, f16* vd, Shared& sh, int buf,
-                                        int e_run) {
+__device__ __forceinline__ void deliver(const Group<D, Q8>& gr, int wave, f16* kd, f16* vd,
+                                        Shared& sh, int buf, int e_run) {
   using C = Cfg<D, Q8>;
+  const int lane = lane_now();
   if constexpr (Q8) {
     uint32_t top = gr.ve[0];
 #pragma unroll
@@ -300,9 +295,9 @@ __device__ __forceinline__ void deliver(const Group<D, Q8>& gr, const Pieces<D, 
       eg = __builtin_amdgcn_readfirstlane(max(e_run, wave_max_i(static_cast<int>(top))));
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
-      const int f = i * kWave + lane, ch = f % C::GCH;
-      if (16 * C::GCH % kWave != 0 && f / C::GCH >= 16) continue;
-      const int R = 16 * wave + pc.row[i];
+      const Piece pc = piece<D, Q8>(i, lane);
+      if (!pc.in) continue;
+      const int ch = pc.k / 16, R = 16 * wave + pc.row;
       const float ks = scale_of(gr.ke[i]);
       const float vs = __uint_as_float(
           static_cast<uint32_t>(max(1, 127 + static_cast<int>(gr.ve[i]) - eg)) << 23);
@@ -554,15 +549,56 @@ __device__ __forceinline__ bool row_place(const Args& a, int64_t tok, int& seq, 
          (static_cast<int64_t>(pos) + a.block_size) / a.block_size <= a.max_blocks;
 }
 
-// All keys of this workgroup's split for its rows, sequence by sequence.
+// This lane's query row (lanes l and l + 32 share one): its token, head, sequence
+// and position; ok: it is written.
+struct Row {
+  int64_t tok;
+  int head, seq, pos;
+  bool ok;
+};
+__device__ __forceinline__ Row row_of(const Args& a, int tile, int kvh, int wave, int lane) {
+  const uint32_t n_rows = static_cast<uint32_t>(a.num_tokens) * a.G;  // below 2^30 + kRows
+  uint32_t rho = static_cast<uint32_t>(tile) * kRows + 32 * wave + (lane & 31);
+  const bool in = rho < n_rows;
+  rho = in ? rho : 0;
+  Row r;
+  r.tok = rho / static_cast<uint32_t>(a.G);
+  r.head = kvh * a.G + static_cast<int>(rho % static_cast<uint32_t>(a.G));
+  r.ok = row_place(a, r.tok, r.seq, r.pos) && in;
+  return r;
+}
+
+// All keys of this workgroup's split for its rows, sequence by sequence.  Rows and Q
+// are read here, so that neither lives on behind the loop.
 template <int D, typename T, bool Q8, bool kAny, bool kCareful>
-__device__ __forceinline__ void walk(const Args& a, f16* ks, f16* vs,
-                                     Shared& sh, int kvh, int split, int wave, int lane,
-                                     bool row_ok, int tseq, int tpos, const Lanes<D>& L,
-                                     const Pieces<D, Q8>& pc, const u32x4 (&qb)[D / 16],
-                                     State<D>& st) {
+__device__ __forceinline__ void walk(const Args& a, f16* ks, f16* vs, Shared& sh, int tile,
+                                     int kvh, int split, int wave, State<D>& st) {
   using C = Cfg<D, Q8>;
-  const int hb = lane >> 5;
+  const int lane = lane_now(), hb = lane >> 5;
+  Lanes<D> L;
+  u32x4 qb[C::NK];
+  int tseq, tpos;
+  bool row_ok;
+  {
+    const Row r = row_of(a, tile, kvh, wave, lane);
+    tseq = r.seq;
+    tpos = r.pos;
+    row_ok = r.ok;
+    const uint16_t* qp = a.q + r.tok * a.q_st + r.head * a.q_sh + hb * (D / 2);
+#pragma unroll
+    for (int s = 0; s < C::NK; ++s)
+      qb[s] = !kAny || hb * (D / 2) + 8 * s < a.hd ? ld16(qp + 8 * s) : u32x4{0u, 0u, 0u, 0u};
+    const int qj = lane & 31;
+#pragma unroll
+    for (int s = 0; s < (Lanes<D>::XOR ? 1 : C::NK); ++s)
+      L.k[s] = qj * C::ROWB + ((hb * (C::CH / 2) + s) ^ swzk<D>(qj)) * 16;
+    const int g16 = lane >> 4, i16 = lane & 15;
+    const int rv = 4 * hb + (i16 >> 2), j4 = i16 & 3;
+#pragma unroll
+    for (int dt = 0; dt < (Lanes<D>::XOR ? 1 : C::NDT); ++dt)
+      L.v[dt] = rv * C::ROWB + ((4 * dt + 2 * (g16 & 1) + (j4 >> 1)) ^ swz<D>(rv)) * 16 +
+                (j4 & 1) * 8;
+  }
   st.m = -INFINITY;
   st.l = 0.f;
   st.e = 0;
@@ -620,14 +656,12 @@ __device__ __forceinline__ void walk(const Args& a, f16* ks, f16* vs,
       Group<D, Q8> gr;
       auto get = [&](int t, int buf) {
         if (t < t_hi)
-          fetch<D, Q8, kAny>(a, bts, kvh, key_of(t) + 16 * wave, rg, wave, lane, pc, w,
-                             ks + buf * C::TILE, vs + buf * C::TILE, gr);
+          fetch<D, Q8, kAny>(a, bts, kvh, key_of(t) + 16 * wave, rg, wave, w, ks + buf * C::TILE, vs + buf * C::TILE, gr);
       };
       // The tile is in LDS: codes converted, direct loads landed, for every wave.
       auto put = [&](int t, int buf) {
         if (t < t_hi)
-          deliver<D, T, Q8>(gr, pc, wave, lane, ks + buf * C::TILE, vs + buf * C::TILE, sh, buf,
-                            e_run);
+          deliver<D, T, Q8>(gr, wave, ks + buf * C::TILE, vs + buf * C::TILE, sh, buf, e_run);
         wait_all();
         __builtin_amdgcn_s_barrier();
         if (Q8 && t < t_hi) {
@@ -668,42 +702,9 @@ prefill_view_kernel(Args a) {
   if (logical >= a.tiles_x * a.kvh) return;
   const int kvh = logical / a.tiles_x, split = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave;
-  const int qj = lane & 31, hb = lane >> 5;
-
-  // This lane's row (lanes l and l + 32 share one).
-  const uint32_t n_rows = static_cast<uint32_t>(a.num_tokens) * a.G;  // below 2^30 + kRows
-  uint32_t rho = static_cast<uint32_t>(logical % a.tiles_x) * kRows + 32 * wave + qj;
-  const bool in = rho < n_rows;
-  rho = in ? rho : 0;
-  const int64_t tok = rho / static_cast<uint32_t>(a.G);
-  const int head = kvh * a.G + static_cast<int>(rho % static_cast<uint32_t>(a.G));
-  int tseq, tpos;
-  const bool row_ok = row_place(a, tok, tseq, tpos) && in;
-  u32x4 qb[C::NK];
-  {
-    const uint16_t* qp = a.q + tok * a.q_st + head * a.q_sh + hb * (D / 2);
-#pragma unroll
-    for (int s = 0; s < C::NK; ++s)
-      qb[s] = !kAny || hb * (D / 2) + 8 * s < a.hd ? ld16(qp + 8 * s) : u32x4{0u, 0u, 0u, 0u};
-  }
-  Lanes<D> L;
-#pragma unroll
-  for (int s = 0; s < (Lanes<D>::XOR ? 1 : C::NK); ++s)
-    L.k[s] = qj * C::ROWB + ((hb * (C::CH / 2) + s) ^ swzk<D>(qj)) * 16;
-  {
-    const int g16 = lane >> 4, i16 = lane & 15;
-    const int r = 4 * hb + (i16 >> 2), j4 = i16 & 3;
-#pragma unroll
-    for (int dt = 0; dt < (Lanes<D>::XOR ? 1 : C::NDT); ++dt)
-      L.v[dt] = r * C::ROWB + ((4 * dt + 2 * (g16 & 1) + (j4 >> 1)) ^ swz<D>(r)) * 16 +
-                (j4 & 1) * 8;
-  }
-  Pieces<D, Q8> pc;
-  pieces_init<D, Q8>(a, wave, lane, pc);
+  const int tile = logical % a.tiles_x;
   State<D> st;
-  walk<D, T, Q8, kAny, false>(a, ks, vs, sh, kvh, split, wave, lane, row_ok, tseq,
-                              tpos, L, pc, qb, st);
+  walk<D, T, Q8, kAny, false>(a, ks, vs, sh, tile, kvh, split, wave, st);
   {
     // An infinity or a NaN in O^T: all over again with care, since it may come from a
     // key that its row does not see.
@@ -712,23 +713,25 @@ prefill_view_kernel(Args a) {
     for (int dt = 0; dt < C::NDT; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = max(top, laundered(st.acc[dt][r]) & 0x7FFFFFFFu);
-    const bool bad = __builtin_amdgcn_ballot_w64(row_ok && top >= 0x7F800000u) != 0;
-    if (lane == 0) sh.bad[wave] = bad;
+    // (Rows that are not written count too: they hold what their garbage gives.)
+    const bool bad = __builtin_amdgcn_ballot_w64(top >= 0x7F800000u) != 0;
+    if (lane_now() == 0) sh.bad[wave] = bad;
     lds_bar();
     int any = 0;
 #pragma unroll
     for (int w = 0; w < kWavesV; ++w) any |= sh.bad[w];
     if (__builtin_amdgcn_readfirstlane(any)) {
-      walk<D, T, Q8, kAny, true>(a, ks, vs, sh, kvh, split, wave, lane, row_ok, tseq,
-                                 tpos, L, pc, qb, st);
+      walk<D, T, Q8, kAny, true>(a, ks, vs, sh, tile, kvh, split, wave, st);
     }
   }
 
   const float l = half_sum(st.l);
-  if (!row_ok) return;
+  const int lane = lane_now(), hb = lane >> 5;
+  const Row r = row_of(a, tile, kvh, wave, lane);
+  if (!r.ok) return;
   float inv = l > 0.f ? 1.f / l : 0.f;
   const float back = Q8 ? scale_of(static_cast<uint32_t>(max(1, st.e))) : 1.f;
-  const int64_t row = tok * a.H + head;
+  const int64_t row = r.tok * a.H + r.head;
   if (a.n_splits > 1) {
     float* dst = a.ws_acc + (row * a.n_splits + split) * D;
 #pragma unroll
@@ -746,7 +749,7 @@ prefill_view_kernel(Args a) {
           laundered(l) != 0u ? st.m + __builtin_log2f(l) : -INFINITY;
     return;
   }
-  uint16_t* op = a.out + tok * a.o_st + head * a.o_sh;
+  uint16_t* op = a.out + r.tok * a.o_st + r.head * a.o_sh;
 #pragma unroll
   for (int dt = 0; dt < C::NDT; ++dt)
 #pragma unroll
