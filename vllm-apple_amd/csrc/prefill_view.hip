@@ -142,18 +142,24 @@ __device__ __forceinline__ int lane_now() {
 // row of its K and V chunk.  16-bit pieces are the ones that the direct load's slot
 // holds.
 struct Piece {
-  int row;
-  uint32_t k, v;
+  uint32_t row, k, v;
   bool in;  // Q8: the piece lies in the group (D = 96 and 32 leave some over)
 };
 template <int D, bool Q8>
-__device__ __forceinline__ Piece piece(int i, int lane) {
+__device__ __forceinline__ Piece piece(uint32_t i, uint32_t lane) {
   using C = Cfg<D, Q8>;
-  const int f = 64 * i + lane, r = f / C::GCH, c = f % C::GCH;
+  uint32_t r, c;
+  if constexpr (kWave % C::GCH == 0) {
+    r = lane / C::GCH + i * (kWave / C::GCH);
+    c = lane % C::GCH;
+  } else {
+    r = (64 * i + lane) / C::GCH;
+    c = (64 * i + lane) % C::GCH;
+  }
   if constexpr (Q8)
-    return {r & 15, 16u * c, 16u * c, r < 16};
+    return {r & 15, 16 * c, 16 * c, r < 16};
   else
-    return {r, 16u * (c ^ swzk<D>(r)), 16u * (c ^ swz<D>(r)), true};
+    return {r, 16 * (c ^ swzk<D>(r)), 16 * (c ^ swz<D>(r)), true};
 }
 
 // Starts the loads of keys k0 .. k0 + 15, this wave's group of a tile.  Rows that no
@@ -202,8 +208,8 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
     for (int i = 0; i < C::NI; ++i) {
       const Piece pc = piece<D, Q8>(i, lane);
       const bool good = row_at(pc.row, p, rin) && pc.in;
-      const char* ks = kb + p * a.k_sb + rin * a.k_st + pc.k;
-      const char* vs = vb + p * a.v_sb + rin * a.v_st + pc.v;
+      const char* ks = kb + p * a.k_sb + static_cast<int64_t>(rin) * a.k_st + pc.k;
+      const char* vs = vb + p * a.v_sb + static_cast<int64_t>(rin) * a.v_st + pc.v;
       const bool kin = good && pc.k < row_bytes, vin = good && pc.v < row_bytes;
       if constexpr (Q8) {
         gr.k[i] = kin ? ld16(ks) : z;
@@ -259,8 +265,14 @@ __device__ __forceinline__ void fetch(const Args& a, const int32_t* bts, int kvh
 #pragma unroll
       for (int i = 0; i < C::NI; ++i) {
         const Piece pc = piece<D, Q8>(i, lane);
-        dma16s(kb, pc.row * a.k_st + pc.k, ka + 1024 * i);
-        dma16s(vb, pc.row * a.v_st + pc.v, va + 1024 * i);
+        if constexpr (kWave % C::GCH == 0) {  // rows of load i: the first load's, further on
+          const uint32_t up = i * (kWave / C::GCH), r0 = pc.row - up;
+          dma16s(kb + up * a.k_st, r0 * a.k_st + pc.k, ka + 1024 * i);
+          dma16s(vb + up * a.v_st, r0 * a.v_st + pc.v, va + 1024 * i);
+        } else {
+          dma16s(kb, pc.row * a.k_st + pc.k, ka + 1024 * i);
+          dma16s(vb, pc.row * a.v_st + pc.v, va + 1024 * i);
+        }
       }
       return;
     }
@@ -361,14 +373,14 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
   using P8 = typename Elem<PT>::x8;
   using X8 = typename Elem<T>::x8;
   constexpr bool kPair = !Q8 && Elem<T>::kSplitP;
-  // By position, does every row of the wave see the whole tile, or none of it any?
+  // Does every row of the wave see the whole tile, by position?  (A wave that sees
+  // nothing of it goes through all the same: a way around the products would keep a
+  // second set of accumulators, and a copy of them per tile.)
   uint64_t seen = ~0ull;
   const bool inside = see.lim - key0 >= kKT - 1 && (see.lo <= key0 || a.first - key0 >= kKT);
   const bool whole = __builtin_amdgcn_ballot_w64(inside) == ~0ull;
-  if (!whole) {
+  if (!whole)
     seen = low64(see.lim + 1 - key0) & (~low64(see.lo - key0) | low64(a.first - key0));
-    if (__builtin_amdgcn_ballot_w64(seen != 0) == 0) return;
-  }
   // What the tile holds, and its exponents: used behind the first product.
   const uint64_t held = sh.ok[buf];
   const uint32_t held_e = Q8 ? sh.ev[buf] : 0;
