@@ -66,11 +66,18 @@ struct Args {
   int part_tiles, max_parts;
   int lds_main;
   int window, first;
-  int64_t num_blocks;
-  int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;        // bytes
+  int bs_shift;         // log2(block_size) where it is a power of two, else -1
+  uint32_t num_blocks;  // at most 2^31: block ids are 32-bit
+  // Bytes.  Block strides are below 2^32 and offsets inside a block 32-bit.
+  uint32_t k_sb, k_st, v_sb, v_st;
+  int64_t k_sh, v_sh;
   int64_t ke_sb, ke_sh, ke_st, ve_sb, ve_sh, ve_st;  // bytes
   int64_t q_st, q_sh, o_st, o_sh;                    // elements
 };
+
+__device__ __forceinline__ int block_of(const Args& a, int key) {
+  return a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
+}
 
 template <int D, bool Q8>
 struct Cfg {
@@ -144,6 +151,7 @@ struct LaneMap {
   int vrow[C::VLD];
   uint32_t koff, voff[C::VLD];  // byte offsets inside a 16-row group / from its rows
   uint32_t wlds[C::VLD];        // element offset in the LDS tile
+  uint32_t keoff, veoff;        // Q8: byte offset of row lane % 16's exponents
   uint32_t trbase;
   int trsw;
   uint32_t kval, vval;  // kAny: bit i set where piece i lies below hd
@@ -168,31 +176,36 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
   const int c16 = lane & 15;
   uint32_t ok = 0;
   if (!kAny || a.block_size % 16 == 0) {
-    int64_t kr[C::NG], vr[C::NG], phys[C::NG];
-    int rin[C::NG];
+    uint64_t kr[C::NG], vr[C::NG];
+    uint64_t ker[C::NG], ver[C::NG];
 #pragma unroll
     for (int grp = 0; grp < C::NG; ++grp) {
       const int tok = tok0 + 16 * grp;
-      const int bi = tok / a.block_size;
-      rin[grp] = tok - bi * a.block_size;
+      const int bi = block_of(a, tok);
+      uint32_t rin = tok - bi * a.block_size;
       // The second group of a window's last tile may lie past the 64 entries.
-      int64_t p = bi - blk0 < kWave ? __builtin_amdgcn_readlane(vals, bi - blk0) : -1;
-      if (p >= 0 && p < a.num_blocks) {
+      uint32_t p = bi - blk0 < kWave
+                       ? static_cast<uint32_t>(__builtin_amdgcn_readlane(vals, bi - blk0))
+                       : ~0u;
+      if (p < a.num_blocks) {
         ok |= 0xFFFFu << (16 * grp);
       } else {
         p = 0;
-        rin[grp] = 0;
+        rin = 0;
       }
-      phys[grp] = p;
-      kr[grp] = p * a.k_sb + rin[grp] * a.k_st;
-      vr[grp] = p * a.v_sb + rin[grp] * a.v_st;
+      kr[grp] = static_cast<uint64_t>(p) * a.k_sb + rin * a.k_st;
+      vr[grp] = static_cast<uint64_t>(p) * a.v_sb + rin * a.v_st;
+      if constexpr (Q8) {
+        ker[grp] = p * a.ke_sb + kvh * a.ke_sh + rin * a.ke_st;
+        ver[grp] = p * a.ve_sb + kvh * a.ve_sh + rin * a.ve_st;
+      }
     }
 #pragma unroll
     for (int grp = 0; grp < C::NG; ++grp)
 #pragma unroll
       for (int i = 0; i < C::KL; ++i) {
         const KP* src = reinterpret_cast<const KP*>(
-            kb + kr[grp] + m.koff + i * (Q8 ? (C::WIDE ? 64 : 32) : 64));
+            kb + kr[grp] + i * (Q8 ? (C::WIDE ? 64 : 32) : 64) + m.koff);
         if (kAny && !((m.kval >> i) & 1u))
           t.k[grp * C::KL + i] = KP{};
         else
@@ -200,7 +213,7 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
       }
 #pragma unroll
     for (int i = 0; i < C::VLD; ++i) {
-      int64_t r;
+      uint64_t r;
       if constexpr (C::NG == 1)
         r = vr[0];
       else if constexpr (C::VUNI)
@@ -213,11 +226,9 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
         t.v[i] = ld16_stream(vb + r + m.voff[i]);
     }
     if constexpr (Q8) {
-      const int grp = (lane >> 4) & 1;
-      const int64_t p = grp ? phys[C::NG - 1] : phys[0];
-      const int r = (grp ? rin[C::NG - 1] : rin[0]) + c16;
-      t.ke = a.ke[p * a.ke_sb + kvh * a.ke_sh + r * a.ke_st];
-      t.ve = a.ve[p * a.ve_sb + kvh * a.ve_sh + r * a.ve_st];
+      const bool up = lane & 16;
+      t.ke = a.ke[(up ? ker[C::NG - 1] : ker[0]) + m.keoff];
+      t.ve = a.ve[(up ? ver[C::NG - 1] : ver[0]) + m.veoff];
     }
     return ok;
   }
@@ -227,7 +238,7 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
     const int bi = tok / a.block_size, w = bi - blk0;
     phys = __shfl(vals, min(w, kWave - 1), kWave);
     rin = tok - bi * a.block_size;
-    const bool good = w < kWave && phys >= 0 && phys < a.num_blocks;
+    const bool good = w < kWave && phys >= 0 && static_cast<uint32_t>(phys) < a.num_blocks;
     if (!good) {
       phys = 0;
       rin = 0;
@@ -240,7 +251,8 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
     int r;
     const bool good = row_at(16 * grp + c16, p, r);
     ok |= (static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(good)) & 0xFFFFu) << (16 * grp);
-    const uint8_t* row = kb + p * a.k_sb + r * a.k_st + (m.koff - c16 * (uint32_t)a.k_st);
+    const uint8_t* row =
+        kb + p * a.k_sb + static_cast<int64_t>(r) * a.k_st + (m.koff - c16 * a.k_st);
 #pragma unroll
     for (int i = 0; i < C::KL; ++i) {
       const KP* src = reinterpret_cast<const KP*>(row + i * (Q8 ? (C::WIDE ? 64 : 32) : 64));
@@ -253,7 +265,7 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
     int r;
     row_at(m.vrow[i], p, r);
     const int ch = (i * kWave + lane) % C::VCH;
-    t.v[i] = ((m.vval >> i) & 1u) ? ld16(vb + p * a.v_sb + r * a.v_st + ch * 16)
+    t.v[i] = ((m.vval >> i) & 1u) ? ld16(vb + p * a.v_sb + static_cast<int64_t>(r) * a.v_st + ch * 16)
                                   : u32x4{0u, 0u, 0u, 0u};
   }
   if constexpr (Q8) {
@@ -378,20 +390,24 @@ __device__ __forceinline__ void decode_range(const Args& a, unsigned char* smem,
                                              int qh0, int nh, const Span& sp, int t0, int t1,
                                              const RangeOut& ro, bool trailing_barrier) {
   using C = Cfg<D, Q8>;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  // Uniform, so that tiles, blocks and masks are the scalar unit's.
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
   const int c16 = lane & 15, g = lane >> 4;
   const int per = (t1 - t0 + NW - 1) / NW;
   const int jb = min(t0 + wave * per, t1), je = min(jb + per, t1);
 
   LaneMap<D, Q8> m;
-  m.koff = c16 * static_cast<uint32_t>(a.k_st) + g * (C::WIDE ? 16 : 8);
+  m.koff = c16 * a.k_st + g * (C::WIDE ? 16 : 8);
+  m.keoff = c16 * static_cast<uint32_t>(a.ke_st);
+  m.veoff = c16 * static_cast<uint32_t>(a.ve_st);
   m.kval = 0;
   m.vval = 0;
 #pragma unroll
   for (int i = 0; i < C::VLD; ++i) {
     const int f = i * kWave + lane, row = f / C::VCH, ch = f % C::VCH;
     m.vrow[i] = row;
-    m.voff[i] = (row & 15) * static_cast<uint32_t>(a.v_st) + ch * 16;
+    m.voff[i] = (row & 15) * a.v_st + ch * 16;
     const int ch8 = Q8 ? 2 * ch : ch;
     m.wlds[i] = row * D + ((ch8 ^ swz<D>(row)) * 8);
     m.vval |= (ch * C::VPER < a.hd ? 1u : 0u) << i;
@@ -429,7 +445,7 @@ __device__ __forceinline__ void decode_range(const Args& a, unsigned char* smem,
   // within 64 table entries (one per lane); loads go one tile ahead of the math.
   for (int cb = jb; cb < je;) {
     const int r0 = sp.real(cb);
-    const int blk0 = r0 * C::R / a.block_size;
+    const int blk0 = block_of(a, r0 * C::R);
     const int64_t fits = (static_cast<int64_t>(blk0) + kWave) * a.block_size / C::R - r0;
     int ce = cb < sp.nf ? min(je, sp.nf) : je;
     // A tile that crosses the 64th entry is the next run's, unless it is the first
@@ -880,10 +896,15 @@ extern "C" int vaa_paged_attention_decode_view(const vaa_attn_params* p, const v
   a.max_parts = sp.max_parts;
   a.window = view->window;
   a.first = view->first_tokens;
-  a.num_blocks = p->num_blocks;
+  a.bs_shift = (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
+  a.num_blocks = static_cast<uint32_t>(std::min<int64_t>(p->num_blocks, int64_t{1} << 31));
   const int w = q8 ? 1 : 2;  // bytes of a cached value
-  a.k_sb = p->k_stride_block * w; a.k_sh = p->k_stride_head * w; a.k_st = p->k_stride_token * w;
-  a.v_sb = p->v_stride_block * w; a.v_sh = p->v_stride_head * w; a.v_st = p->v_stride_token * w;
+  a.k_sb = static_cast<uint32_t>(p->k_stride_block * w);
+  a.v_sb = static_cast<uint32_t>(p->v_stride_block * w);
+  a.k_st = static_cast<uint32_t>(p->k_stride_token * w);
+  a.v_st = static_cast<uint32_t>(p->v_stride_token * w);
+  a.k_sh = p->k_stride_head * w;
+  a.v_sh = p->v_stride_head * w;
   a.ke_sb = view->ke_stride_block; a.ke_sh = view->ke_stride_head;
   a.ke_st = view->ke_stride_token;
   a.ve_sb = view->ve_stride_block; a.ve_sh = view->ve_stride_head;

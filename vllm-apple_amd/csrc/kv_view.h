@@ -48,6 +48,8 @@ inline int check_view(const char* what, const vaa_attn_params* p, const vaa_kv_v
                             view->ve_stride_block, view->ve_stride_head, view->ve_stride_token};
     for (int64_t s : exps)
       if (s < 0) return fail(VAA_ERR_INVALID_ARG, "%s: negative exponent stride", what);
+    if (view->ke_stride_token >= (int64_t{1} << 24) || view->ve_stride_token >= (int64_t{1} << 24))
+      return fail(VAA_ERR_INVALID_ARG, "%s: exponent token stride too large", what);
   }
   // Offsets inside a block are 32-bit bytes.
   if (p->k_stride_block >= (int64_t{1} << 31) || p->v_stride_block >= (int64_t{1} << 31) ||
