@@ -464,8 +464,8 @@ int vaa_kv_read_slots_q8(const vaa_attn_params* p, const vaa_kv_view* view,
  * (there is no fused write).  Arguments, guards and workspace as there, with two
  * differences: partition_size > 0 and the automatic one count the tokens that
  * are seen, and VAA_PARTITION_BALANCED_SHARED is VAA_ERR_UNSUPPORTED.
- * VAA_CACHE_E4M3: head_size a multiple of 16, codes 16-byte aligned with strides
- * that are multiples of 16; K, Q and V enter the products as p->dtype, which holds
+ * p->scale must be positive.  VAA_CACHE_E4M3: head_size a multiple of 16, codes
+ * 16-byte aligned with strides that are multiples of 16; K, Q and V enter the products as p->dtype, which holds
  * every value of a row written from it exactly (fp16: but for those below its
  * normal range).
  */

@@ -97,9 +97,13 @@ struct Cfg {
   static constexpr bool VUNI = NG == 1 || (kWave % VCH == 0 && 16 % (kWave / VCH) == 0);
 };
 
+// Chunk swizzle of the V tile in LDS: physical 16-byte chunk = logical ^ swz(row).
+// Four rows side by side, which a transposing read takes together, differ in their
+// chunk pair; two rows side by side, which a write of two chunks a lane takes
+// together, in the chunk of the pair.
 template <int D>
 __device__ __forceinline__ int swz(int row) {
-  return (D == 64 || D == 128) ? ((row >> 2) & 3) << 1 : 0;
+  return (D == 64 || D == 128) ? ((row & 3) << 1) | (row & 1) : 0;
 }
 
 template <bool kWidePiece>
@@ -278,9 +282,9 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
   return ok;
 }
 
-// One tile of math; bit r of seen: row r counts.
-template <int D, typename T, bool Q8>
-__device__ __forceinline__ void tile_math(const LaneMap<D, Q8>& m, const Tile<D, Q8>& t,
+// One tile of math; bit r of seen: row r counts (kMask false: all do).
+template <int D, typename T, bool Q8, bool kMask>
+__device__ __forceinline__ void tile_product(const LaneMap<D, Q8>& m, const Tile<D, Q8>& t,
                                           const u32x4* qb, T* vt, uint32_t seen, int lane,
                                           float scale_log2, float& m_run, float& l_part,
                                           f32x4* acc) {
@@ -292,12 +296,13 @@ __device__ __forceinline__ void tile_math(const LaneMap<D, Q8>& m, const Tile<D,
   // V to LDS; rows that do not count become zeros, whatever they hold.
 #pragma unroll
   for (int i = 0; i < C::VLD; ++i) {
-    const bool in = (seen >> m.vrow[i]) & 1u;
+    const bool in = !kMask || ((seen >> m.vrow[i]) & 1u);
     if constexpr (Q8) {
       const float s = scale_of(__shfl(t.ve, m.vrow[i], kWave));
       const u32x4 lo = deq8<T>(t.v[i][0], t.v[i][1], s), hi = deq8<T>(t.v[i][2], t.v[i][3], s);
       *reinterpret_cast<u32x4*>(vt + m.wlds[i]) = in ? lo : zero;
-      *reinterpret_cast<u32x4*>(vt + m.wlds[i] + 8) = in ? hi : zero;
+      *reinterpret_cast<u32x4*>(vt + (m.wlds[i] ^ (C::SWZ ? 8 : 0)) + (C::SWZ ? 0 : 8)) =
+          in ? hi : zero;
     } else {
       *reinterpret_cast<u32x4*>(vt + m.wlds[i]) = in ? t.v[i] : zero;
     }
@@ -324,17 +329,16 @@ __device__ __forceinline__ void tile_math(const LaneMap<D, Q8>& m, const Tile<D,
     }
   }
   // Online softmax, log2 domain: lane = head, tokens 16 grp + 4g + r.
-  float x[C::NG][4];
   float mx = -INFINITY;
 #pragma unroll
   for (int grp = 0; grp < C::NG; ++grp)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      x[grp][r] = ((seen >> (16 * grp + 4 * g + r)) & 1u) ? s4[grp][r] * scale_log2 : -INFINITY;
-      mx = fmaxf(mx, x[grp][r]);
+      if (kMask && !((seen >> (16 * grp + 4 * g + r)) & 1u)) s4[grp][r] = -INFINITY;
+      mx = fmaxf(mx, s4[grp][r]);
     }
   mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, kWave)) * scale_log2;
   const float m_new = fmaxf(m_run, mx);
   if (m_new != m_run) {
     const float alpha = fast_exp2(m_run - m_new);  // 0 when m_run = -inf
@@ -344,15 +348,23 @@ __device__ __forceinline__ void tile_math(const LaneMap<D, Q8>& m, const Tile<D,
     m_run = m_new;
   }
   const float m_sub = m_run == -INFINITY ? 0.f : m_run - kPShift<T>;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef decltype(Elem<T>::from_f(0.f)) E2 __attribute__((ext_vector_type(2)));
   X4 ph[C::NG], pl[C::NG];
 #pragma unroll
   for (int grp = 0; grp < C::NG; ++grp)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float p = fast_exp2(x[grp][r] - m_sub);
-      ph[grp][r] = Elem<T>::from_f(p);
-      pl[grp][r] = Elem<T>::from_f(p - Elem<T>::to_f(ph[grp][r]));
-      l_part += Elem<T>::to_f(ph[grp][r]) + Elem<T>::to_f(pl[grp][r]);
+    for (int r = 0; r < 4; r += 2) {
+      const f32x2 p = {fast_exp2(fmaf(s4[grp][r], scale_log2, -m_sub)),
+                       fast_exp2(fmaf(s4[grp][r + 1], scale_log2, -m_sub))};
+      const E2 h = __builtin_convertvector(p, E2);
+      const E2 l = __builtin_convertvector(
+          f32x2{p[0] - Elem<T>::to_f(h[0]), p[1] - Elem<T>::to_f(h[1])}, E2);
+      ph[grp][r] = h[0];
+      ph[grp][r + 1] = h[1];
+      pl[grp][r] = l[0];
+      pl[grp][r + 1] = l[1];
+      l_part += p[0] + p[1];
     }
   // O^T += V^T P^T; one transposing read gives a lane V[16 grp + 4g + r][16 dt + c16].
 #pragma unroll
@@ -375,6 +387,17 @@ __device__ __forceinline__ void tile_math(const LaneMap<D, Q8>& m, const Tile<D,
       acc[dt] = Elem<T>::mfma16x16x16(va[0], pl[0], acc[dt]);
     }
   }
+}
+
+template <int D, typename T, bool Q8>
+__device__ __forceinline__ void tile_math(const LaneMap<D, Q8>& m, const Tile<D, Q8>& t,
+                                          const u32x4* qb, T* vt, uint32_t seen, int lane,
+                                          float scale_log2, float& m_run, float& l_part,
+                                          f32x4* acc) {
+  if (seen == low_bits(Cfg<D, Q8>::R))
+    tile_product<D, T, Q8, false>(m, t, qb, vt, seen, lane, scale_log2, m_run, l_part, acc);
+  else
+    tile_product<D, T, Q8, true>(m, t, qb, vt, seen, lane, scale_log2, m_run, l_part, acc);
 }
 
 // Where the result of one (sequence, kv head, range of tiles) goes.
@@ -419,8 +442,8 @@ __device__ __forceinline__ void decode_range(const Args& a, unsigned char* smem,
     m.kval |= ((Q8 && C::WIDE ? 64 * i + 16 * g : 32 * i + 8 * g) < a.hd ? 1u : 0u) << i;
   {
     const int row = 4 * g + (c16 >> 2), j = c16 & 3;
-    m.trsw = swz<D>(row);
-    m.trbase = row * D + (j >> 1) * 8 + (j & 1) * 4;
+    m.trsw = swz<D>(row) & ~1;
+    m.trbase = row * D + ((j >> 1) ^ (swz<D>(row) & 1)) * 8 + (j & 1) * 4;
   }
 
   // Q^T as the B operand, its dims in the order of K's pieces.

@@ -16,6 +16,10 @@ inline int check_view(const char* what, const vaa_attn_params* p, const vaa_kv_v
   if (!valid_dtype(p->dtype))
     return fail(VAA_ERR_UNSUPPORTED, "%s: dtype=%d (VAA_DTYPE_F16 or VAA_DTYPE_BF16)", what,
                 p->dtype);
+  // The running maximum is taken over the products, before the scale.
+  if (!(p->scale > 0.f && p->scale < 3.0e38f))
+    return fail(VAA_ERR_INVALID_ARG, "%s: scale=%g must be positive and finite", what,
+                static_cast<double>(p->scale));
   if (p->block_size <= 0)
     return fail(VAA_ERR_INVALID_ARG, "%s: block_size=%d must be positive", what, p->block_size);
   if (p->num_kv_heads <= 0 || p->num_query_heads <= 0 ||
