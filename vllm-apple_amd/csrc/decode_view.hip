@@ -282,6 +282,19 @@ __device__ __forceinline__ uint32_t issue(const Args& a, const LaneMap<D, Q8>& m
   return ok;
 }
 
+// The maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48, in all of them: the swaps
+// exchange odd rows of 16 lanes (halves of the wave) of one operand with even rows
+// (the lower half) of the other, so with x in both the two results hold x and its
+// partner's x.  In the VALU: no LDS round trip between the two products.
+__device__ __forceinline__ float groups_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // One tile of math; bit r of seen: row r counts (kMask false: all do).
 template <int D, typename T, bool Q8, bool kMask>
 __device__ __forceinline__ void tile_product(const LaneMap<D, Q8>& m, const Tile<D, Q8>& t,
@@ -337,8 +350,7 @@ __device__ __forceinline__ void tile_product(const LaneMap<D, Q8>& m, const Tile
       if (kMask && !((seen >> (16 * grp + 4 * g + r)) & 1u)) s4[grp][r] = -INFINITY;
       mx = fmaxf(mx, s4[grp][r]);
     }
-  mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, kWave)) * scale_log2;
+  mx = groups_max(mx) * scale_log2;
   const float m_new = fmaxf(m_run, mx);
   if (m_new != m_run) {
     const float alpha = fast_exp2(m_run - m_new);  // 0 when m_run = -inf
