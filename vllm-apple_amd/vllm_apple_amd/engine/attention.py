@@ -7,6 +7,11 @@ encode_prefill       (attention.py:290-367): token-parallel semantics of
     paged_attention_v2_prefill -- token t attends to [0, positions[t]] of
     sequence token_to_seq[t] -- on the MFMA prefill kernel.  The tokens' K/V
     must already be in the cache (KVWriteOp.encode_prefill).
+
+Each takes, behind the reference's arguments, a sliding window with visible first
+tokens (window, first_tokens) and the exponents of a quantised cache
+(key_exps_buffer, value_exps_buffer, [num_blocks, KV, block_size] uint8): see
+kernels.paged_decode and paged_prefill.  The reference has neither.
 """
 from __future__ import annotations
 
@@ -134,6 +139,12 @@ class PagedAttentionOp:
             raise ValueError("cache buffer size is not a whole number of blocks")
         return buf.reshape(-1, self.num_kv_heads, self.block_size, self.head_size)
 
+    def _exps(self, buf: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """A K or V exponent buffer as [num_blocks, KV, bs]."""
+        if buf is None or buf.dim() == 3:
+            return buf
+        return buf.reshape(-1, self.num_kv_heads, self.block_size)
+
     def fused_params(self, num_seqs: int, max_seq_len: int,
                      max_blocks_per_seq: int) -> FusedAttentionParams:
         return FusedAttentionParams(
@@ -151,7 +162,9 @@ class PagedAttentionOp:
                        positions_buffer: torch.Tensor, output_buffer: torch.Tensor,
                        num_tokens: int, num_seqs: int, max_seq_len: int,
                        max_blocks_per_seq: int, query_offset: int = 0,
-                       output_offset: int = 0) -> None:
+                       output_offset: int = 0, window: int = 0, first_tokens: int = 0,
+                       key_exps_buffer: Optional[torch.Tensor] = None,
+                       value_exps_buffer: Optional[torch.Tensor] = None) -> None:
         stream = resolve_stream(step_ctx)
         H, D = self.num_query_heads, self.head_size
         q = view(query_buffer, query_offset, (num_tokens, H, D))
@@ -161,7 +174,9 @@ class PagedAttentionOp:
         pos = view(positions_buffer, 0, (num_tokens,), torch.int32)
         kernels.paged_prefill(q, self._cache(key_buffer), self._cache(value_buffer), bt, tok,
                               pos, scale=self.scale, layout="kernel", output=out,
-                              stream=stream)
+                              stream=stream, max_seq_len=max_seq_len, window=window,
+                              first_tokens=first_tokens, key_exps=self._exps(key_exps_buffer),
+                              value_exps=self._exps(value_exps_buffer))
 
     def encode_decode_fused(self, step_ctx: Any, query_buffer: torch.Tensor,
                             new_keys_buffer: torch.Tensor, new_values_buffer: torch.Tensor,
@@ -170,7 +185,12 @@ class PagedAttentionOp:
                             output_buffer: torch.Tensor, num_seqs: int, max_seq_len: int,
                             max_blocks_per_seq: int = 0, query_offset: int = 0,
                             new_keys_offset: int = 0, new_values_offset: int = 0,
-                            output_offset: int = 0, partition_size: int = 0) -> None:
+                            output_offset: int = 0, partition_size: int = 0, window: int = 0,
+                            first_tokens: int = 0,
+                            key_exps_buffer: Optional[torch.Tensor] = None,
+                            value_exps_buffer: Optional[torch.Tensor] = None) -> None:
+        """With a window or a quantised cache the write is a launch of its own in front
+        of the decode."""
         stream = resolve_stream(step_ctx)
         if max_blocks_per_seq == 0:
             max_blocks_per_seq = (max_seq_len + self.block_size - 1) // self.block_size
@@ -181,7 +201,17 @@ class PagedAttentionOp:
         out = view(output_buffer, output_offset, (num_seqs, H, D))
         bt = view(block_table_buffer, 0, (num_seqs, max_blocks_per_seq), torch.int32)
         sl = view(seq_lens_buffer, 0, (num_seqs,), torch.int32)
-        kernels.paged_decode(q, self._cache(key_buffer), self._cache(value_buffer), bt, sl,
+        kc, vc = self._cache(key_buffer), self._cache(value_buffer)
+        ke, ve = self._exps(key_exps_buffer), self._exps(value_exps_buffer)
+        if window or first_tokens or ke is not None or ve is not None:
+            kernels.kv_write_decode(nk, nv, kc, vc, bt, sl, key_exps=ke, value_exps=ve,
+                                    layout="kernel", stream=stream)
+            kernels.paged_decode(q, kc, vc, bt, sl, scale=self.scale, max_seq_len=max_seq_len,
+                                 layout="kernel", output=out, partition_size=partition_size,
+                                 stream=stream, window=window, first_tokens=first_tokens,
+                                 key_exps=ke, value_exps=ve)
+            return
+        kernels.paged_decode(q, kc, vc, bt, sl,
                              scale=self.scale, max_seq_len=max_seq_len, layout="kernel",
                              output=out, new_keys=nk, new_values=nv,
                              partition_size=partition_size, stream=stream)
@@ -191,7 +221,9 @@ class PagedAttentionOp:
                       block_table_buffer: torch.Tensor, seq_lens_buffer: torch.Tensor,
                       output_buffer: torch.Tensor, num_seqs: int, max_seq_len: int,
                       max_blocks_per_seq: int = 0, query_offset: int = 0,
-                      output_offset: int = 0, partition_size: int = 0) -> None:
+                      output_offset: int = 0, partition_size: int = 0, window: int = 0,
+                      first_tokens: int = 0, key_exps_buffer: Optional[torch.Tensor] = None,
+                      value_exps_buffer: Optional[torch.Tensor] = None) -> None:
         """Decode over a cache that already holds the new tokens (no fused write)."""
         stream = resolve_stream(step_ctx)
         if max_blocks_per_seq == 0:
@@ -203,7 +235,10 @@ class PagedAttentionOp:
         sl = view(seq_lens_buffer, 0, (num_seqs,), torch.int32)
         kernels.paged_decode(q, self._cache(key_buffer), self._cache(value_buffer), bt, sl,
                              scale=self.scale, max_seq_len=max_seq_len, layout="kernel",
-                             output=out, partition_size=partition_size, stream=stream)
+                             output=out, partition_size=partition_size, stream=stream,
+                             window=window, first_tokens=first_tokens,
+                             key_exps=self._exps(key_exps_buffer),
+                             value_exps=self._exps(value_exps_buffer))
 
     def encode_with_kv_write(self, step_ctx: Any, query_buffer, new_keys_buffer,
                              new_values_buffer, key_buffer, value_buffer, block_table_buffer,

@@ -4,13 +4,15 @@ encode_decode  (kv_write.py:261-334): each sequence's new token at position
                seq_len-1 through block_table (guards of :86-99).
 encode_prefill (kv_write.py:336-402): every token to slot_mapping[t];
                negative slots skipped (:137-138).
-Bit-exact 16-byte copies (kv_write.hip).
+Bit-exact 16-byte copies (kv_write.hip).  With key_exps_buffer and value_exps_buffer
+([num_blocks, KV, block_size] uint8) the cache is quantised and the rows are rounded
+to it (kv_quant.hip); the reference has 16-bit caches only.
 """
 from __future__ import annotations
 
 import struct
 from dataclasses import dataclass
-from typing import Any, Dict
+from typing import Any, Dict, Optional
 
 import torch
 
@@ -56,11 +58,18 @@ class KVWriteOp:
             return buf
         return buf.reshape(-1, self.num_kv_heads, self.block_size, self.head_size)
 
+    def _exps(self, buf: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        if buf is None or buf.dim() == 3:
+            return buf
+        return buf.reshape(-1, self.num_kv_heads, self.block_size)
+
     def encode_decode(self, step_ctx: Any, new_keys_buffer: torch.Tensor,
                       new_values_buffer: torch.Tensor, key_buffer: torch.Tensor,
                       value_buffer: torch.Tensor, block_table_buffer: torch.Tensor,
                       seq_lens_buffer: torch.Tensor, num_seqs: int, new_keys_offset: int = 0,
-                      new_values_offset: int = 0, max_blocks_per_seq: int = 128) -> None:
+                      new_values_offset: int = 0, max_blocks_per_seq: int = 128,
+                      key_exps_buffer: Optional[torch.Tensor] = None,
+                      value_exps_buffer: Optional[torch.Tensor] = None) -> None:
         stream = resolve_stream(step_ctx)
         KV, D = self.num_kv_heads, self.head_size
         nk = view(new_keys_buffer, new_keys_offset, (num_seqs, KV, D))
@@ -68,20 +77,26 @@ class KVWriteOp:
         bt = view(block_table_buffer, 0, (num_seqs, max_blocks_per_seq), torch.int32)
         sl = view(seq_lens_buffer, 0, (num_seqs,), torch.int32)
         kernels.kv_write_decode(nk, nv, self._cache(key_buffer), self._cache(value_buffer), bt,
-                                sl, layout="kernel", stream=stream)
+                                sl, key_exps=self._exps(key_exps_buffer),
+                                value_exps=self._exps(value_exps_buffer), layout="kernel",
+                                stream=stream)
 
     def encode_prefill(self, step_ctx: Any, new_keys_buffer: torch.Tensor,
                        new_values_buffer: torch.Tensor, key_buffer: torch.Tensor,
                        value_buffer: torch.Tensor, slot_mapping_buffer: torch.Tensor,
                        num_tokens: int, new_keys_offset: int = 0,
-                       new_values_offset: int = 0) -> None:
+                       new_values_offset: int = 0,
+                       key_exps_buffer: Optional[torch.Tensor] = None,
+                       value_exps_buffer: Optional[torch.Tensor] = None) -> None:
         stream = resolve_stream(step_ctx)
         KV, D = self.num_kv_heads, self.head_size
         nk = view(new_keys_buffer, new_keys_offset, (num_tokens, KV, D))
         nv = view(new_values_buffer, new_values_offset, (num_tokens, KV, D))
         sm = slot_mapping_buffer.reshape(-1)[:num_tokens]
         kernels.kv_write_slots(nk, nv, self._cache(key_buffer), self._cache(value_buffer), sm,
-                               layout="kernel", stream=stream)
+                               key_exps=self._exps(key_exps_buffer),
+                               value_exps=self._exps(value_exps_buffer), layout="kernel",
+                               stream=stream)
 
     def get_params_dict(self) -> Dict[str, Any]:
         return {

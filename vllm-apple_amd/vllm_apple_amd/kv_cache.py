@@ -13,6 +13,10 @@ The validation methods keep the reference's rules and messages
 run on host (CPU) tensors/arrays, before a step is enqueued, exactly as the
 reference validates at its step boundary; device tensors are copied to the
 host first (one synchronisation, the caller's choice).
+
+A descriptor of dtype torch.float8_e4m3fn makes a quantised cache: the codes, and one
+exponent byte a row beside them (get_exponents; kernels.py has the format).  The
+reference has no such cache.
 """
 from __future__ import annotations
 
@@ -50,12 +54,18 @@ class KVCacheDescriptor:
             raise ValueError(f"head_size must be 32/64/96/128, got {self.head_size}")
 
     @property
+    def quantised(self) -> bool:
+        """e4m3 codes with an exponent byte a row."""
+        return self.dtype == kernels.QUANT_DTYPE
+
+    @property
     def block_size_bytes(self) -> int:
         """Bytes of one block of one layer, K and V together: two
         [KV, bs, D] tiles of the cache's element type (2 bytes for fp16 and
-        bf16 alike)."""
+        bf16 alike), and a quantised cache's exponents."""
         elems = self.num_kv_heads * self.block_size * self.head_size
-        return 2 * elems * torch.empty((), dtype=self.dtype).element_size()
+        exps = self.num_kv_heads * self.block_size if self.quantised else 0
+        return 2 * (elems * torch.empty((), dtype=self.dtype).element_size() + exps)
 
     @property
     def total_cache_bytes(self) -> int:
@@ -84,7 +94,12 @@ class HipKVCache:
         shape = (descriptor.num_layers, 2, descriptor.num_blocks, descriptor.num_kv_heads,
                  descriptor.block_size, descriptor.head_size)
         alloc = torch.zeros if zero else torch.empty
-        self._storage = alloc(shape, dtype=descriptor.dtype, device=dev)
+        self._exponents = None
+        if descriptor.quantised:
+            self._storage = alloc(shape, dtype=torch.uint8, device=dev).view(descriptor.dtype)
+            self._exponents = alloc(shape[:-1], dtype=torch.uint8, device=dev)
+        else:
+            self._storage = alloc(shape, dtype=descriptor.dtype, device=dev)
         self._strides = {
             "block": descriptor.num_kv_heads * descriptor.block_size * descriptor.head_size,
             "head": descriptor.block_size * descriptor.head_size,
@@ -113,6 +128,13 @@ class HipKVCache:
     def get_buffers(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """(key, value) views of one layer, each [nb, KV, bs, D]."""
         return self._storage[layer_idx, 0], self._storage[layer_idx, 1]
+
+    def get_exponents(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(key, value) exponent bytes of one layer of a quantised cache, each
+        [nb, KV, bs]."""
+        if self._exponents is None:
+            raise ValueError(f"a cache of {self._desc.dtype} has no exponents")
+        return self._exponents[layer_idx, 0], self._exponents[layer_idx, 1]
 
     def get_key_buffer(self, layer_idx: int) -> torch.Tensor:
         return self._storage[layer_idx, 0]
@@ -185,6 +207,16 @@ class HipKVCache:
             raise ValueError(f"token_offset {token_offset} >= block_size {self._desc.block_size}")
         k, v = self.get_buffers(layer_idx)
         dev = k.device
+        if self._exponents is not None:
+            if block_id < 0 or block_id >= self._desc.num_blocks or token_offset < 0:
+                raise ValueError(f"block {block_id}, offset {token_offset} outside the cache")
+            rows = [torch.as_tensor(t).to(device=dev) for t in (key, value)]
+            rows = [(t if t.dtype in kernels.ATTN_DTYPES else t.half()).contiguous()[None]
+                    for t in rows]
+            slot = torch.tensor([block_id * self._desc.block_size + token_offset], device=dev)
+            ke, ve = self.get_exponents(layer_idx)
+            kernels.kv_write_slots(*rows, k, v, slot, key_exps=ke, value_exps=ve)
+            return
         key = torch.as_tensor(key).to(device=dev, dtype=k.dtype).contiguous()
         value = torch.as_tensor(value).to(device=dev, dtype=k.dtype).contiguous()
         kernels.write_kv_single(k, v, key, value, block_id, token_offset, self._strides["block"],
@@ -198,4 +230,8 @@ class HipKVCache:
         self.write_kv(layer_idx, block_id, off, key, value)
 
     def reset(self) -> None:
+        if self._exponents is not None:
+            self._storage.view(torch.uint8).zero_()
+            self._exponents.zero_()
+            return
         self._storage.zero_()
