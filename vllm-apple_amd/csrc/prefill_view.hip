@@ -11,7 +11,7 @@
 // the rows; each of its 4 waves takes 32 rows.  For each sequence among its tokens
 // (normally one) it walks the 64-key tiles that any of its rows sees: those of the
 // first tokens, then those from the oldest key in a window to the youngest row.
-// Few rows: the tiles are dealt to several workgroups (grid z) and merged.
+// Few rows: the tiles are dealt to several workgroups (grid y) and merged.
 //   S^T[64 keys x 32 rows] = K Q^T,  P = exp2(S scale log2e - m),
 //   O^T[D x 32 rows] += V^T P^T      on 32x32x16 MFMAs; a lane owns one row.
 //
@@ -26,12 +26,21 @@
 // goes into the group's P.
 //
 // 16-bit rows go to LDS by direct loads, as in the paged prefill.
+//
+// Measured (heads 32 on 8 of 128, blocks of 16): 4 x 512 tokens over 2048, e4m3, bf16
+// 117 us, 660 TFLOP/s (62 us at a large product's rate); 2 x 2048 tokens of which each
+// sees a window of 4096 and 4 first tokens, bf16 390 us, 705 TFLOP/s; the same over e4m3
+// rows about as long.  64 accumulators, Q, a tile's scores and P fill the 256 registers
+// that two waves a SIMD leave, so that a wave has 32 rows and each K and V tile is read
+// from LDS once for every 32: LDS reads, the exponentials and the MFMAs take about the
+// same time each, and the two waves hide part of one beneath the other.
 #include "fp8.h"
 #include "kv_view.h"
 #include "prefill_tile.h"
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 namespace vaa {
@@ -43,7 +52,8 @@ constexpr int kThreadsV = kWavesV * kWave;
 constexpr int kKT = 64;       // keys per tile: a 16-key group per wave
 constexpr int kXcds = 8;
 constexpr int kMaxSplits = 64;
-constexpr int kMinSplitTiles = 4;   // least tiles of a split
+// A tile's time in the partials that are written and read back in it: 1.5 us, 2 MB/us.
+constexpr int64_t kTileBytes = 3 << 20;
 constexpr float kRescale = 8.f;     // lazy rescale: P stays below 2^8
 
 struct Args {
@@ -400,6 +410,9 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[j][r] = 0.f;
+  // Products go before the other workgroup's exponentials: 4 x 512 over 2048, 16-bit
+  // fp16 115 -> 109 us with this and P beneath the products.
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < NKR; ++i) {
     if (i + kAheadK < NKR) kread(i + kAheadK);
@@ -407,6 +420,7 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
                                      __builtin_bit_cast(X8, qb[i >> 1]), s[i & 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(0);
   X4 vlo[NPV], vhi[NPV];
   auto vread = [&](int i) {
     const int g = i / C::NDT, dt = i % C::NDT;
@@ -456,61 +470,47 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
     }
     even = ev == static_cast<uint32_t>(st.e) * 0x01010101u;
   }
+  if (!even) {
+    // A tile that raises E: the product takes P 2^(E_g - E), the sum P itself.
+    float l = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) l += fast_exp2(fmaf(s[j][r], a.scale_log2, -sub));
+    st.l += l;
+  }
   P8 pb[4], pl[4];
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef decltype(Elem<PT>::from_f(0.f)) E2 __attribute__((ext_vector_type(2)));
-  // P of the group's values r, r + 1, to its pair of 16-bit values.
-  auto put = [&](int g, int i, f32x2 p) {
+  float l0 = 0.f, l1 = 0.f;
+  // P of the lane's pair i of group g.
+  auto put = [&](int g, int i) {
+    float sg = sub;
+    if constexpr (Q8) sg += static_cast<float>(st.e - static_cast<int>((ev >> (8 * g)) & 255));
+    const int j = g >> 1, r = 8 * (g & 1) + 2 * i;
+    const f32x2 p = {fast_exp2(fmaf(s[j][r], a.scale_log2, -sg)),
+                     fast_exp2(fmaf(s[j][r + 1], a.scale_log2, -sg))};
     const E2 h = __builtin_convertvector(p, E2);
-    pb[g][i] = h[0];
-    pb[g][i + 1] = h[1];
+    pb[g][2 * i] = h[0];
+    pb[g][2 * i + 1] = h[1];
+    float& l = i & 1 ? l1 : l0;
     if constexpr (kPair) {
       const f32x2 back = {Elem<PT>::to_f(h[0]), Elem<PT>::to_f(h[1])};
-      const E2 l = __builtin_convertvector(f32x2{p[0] - back[0], p[1] - back[1]}, E2);
-      pl[g][i] = l[0];
-      pl[g][i + 1] = l[1];
-      st.l += p[0] + p[1];
-    }
-  };
-  if (even) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2)
-        put(2 * j + (r >> 3), r & 7,
-            f32x2{fast_exp2(fmaf(s[j][r], a.scale_log2, -sub)),
-                  fast_exp2(fmaf(s[j][r + 1], a.scale_log2, -sub))});
-  } else {
-    // A tile that raises E: the sum takes P itself, the product P 2^(E_g - E).
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const int eg = (ev >> (8 * (2 * j + (r >> 3)))) & 255;
-        const float w = __uint_as_float(static_cast<uint32_t>(max(1, 127 + eg - st.e)) << 23);
-        const f32x2 p = {fast_exp2(fmaf(s[j][r], a.scale_log2, -sub)),
-                         fast_exp2(fmaf(s[j][r + 1], a.scale_log2, -sub))};
-        st.l += p[0] + p[1];
-        put(2 * j + (r >> 3), r & 7, f32x2{p[0] * w, p[1] * w});
-      }
-  }
-  if constexpr (!kPair) {
-    // The sum takes P as the product sees it, two values per v_dot2_f32_f16.
-    if (even) {
+      const E2 lo = __builtin_convertvector(f32x2{p[0] - back[0], p[1] - back[1]}, E2);
+      pl[g][2 * i] = lo[0];
+      pl[g][2 * i + 1] = lo[1];
+      l += p[0] + p[1];
+    } else {
+      // The sum takes P as the product sees it, two values per v_dot2_f32_f16.
       typedef _Float16 h2 __attribute__((ext_vector_type(2)));
       const h2 one = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          l0 = __builtin_amdgcn_fdot2(h2{pb[g][i], pb[g][i + 1]}, one, l0, false);
-          l1 = __builtin_amdgcn_fdot2(h2{pb[g][i + 2], pb[g][i + 3]}, one, l1, false);
-        }
-      st.l += l0 + l1;
+      l = __builtin_amdgcn_fdot2(h2{h[0], h[1]}, one, l, false);
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) put(0, i);
   __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < NPV; ++i) {
     if (i + kAheadV < NPV) vread(i + kAheadV);
@@ -549,8 +549,14 @@ __device__ __forceinline__ void tile_math(const Args& a, const f16* kt, const f1
     }
     st.acc[dt] = Elem<PT>::mfma32x32x16(va, pb[g], st.acc[dt]);
     if constexpr (kPair) st.acc[dt] = Elem<PT>::mfma32x32x16(va, pl[g], st.acc[dt]);
+    // The next group's P beneath this one's products.
+    if (g < 3)
+#pragma unroll
+      for (int e = 4 * dt / C::NDT; e < 4 * (dt + 1) / C::NDT; ++e) put(g + 1, e);
     __builtin_amdgcn_sched_barrier(0);
   }
+  if (even) st.l += l0 + l1;
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // A query row's sequence and position; false where the row is left unwritten.
@@ -786,17 +792,40 @@ __global__ void __launch_bounds__(256) prefill_view_merge_kernel(Args a) {
   if (tok >= static_cast<uint32_t>(a.num_tokens) || d >= a.hd) return;
   int seq, pos;
   if (!row_place(a, tok, seq, pos)) return;
+  const float* lse = a.ws_lse + row * a.n_splits;
+  const float* src = a.ws_acc + row * a.n_splits * D + d;
+  constexpr int kAtOnce = 8;  // loads in flight: the kernel is bound by their latency
   float M = -INFINITY, den = 0.f;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  for (int z = 0; z < a.n_splits; ++z) {
-    const float lse = a.ws_lse[row * a.n_splits + z];
-    const f32x4 o = *reinterpret_cast<const f32x4*>(a.ws_acc + (row * a.n_splits + z) * D + d);
-    if (laundered(lse) == 0xFF800000u) continue;  // -inf; a NaN goes on
-    const float Mn = fmaxf(M, lse);
-    const float so = fast_exp2(M - Mn), sn = fast_exp2(lse - Mn);
-    num = num * so + o * sn;
-    den = den * so + sn;
-    M = Mn;
+  for (int z0 = 0; z0 < a.n_splits; z0 += kAtOnce) {
+    float x[kAtOnce];
+    f32x4 o[kAtOnce];  // zeros of a split that saw nothing
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int z = min(z0 + i, a.n_splits - 1);
+      x[i] = lse[z];
+      o[i] = *reinterpret_cast<const f32x4*>(src + z * D);
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (z0 + i >= a.n_splits) {  // the last one again: 0 * inf is not nothing
+        x[i] = -INFINITY;
+        o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      top = fmaxf(top, x[i]);
+    }
+    const float base = top == -INFINITY ? 0.f : top, so = fast_exp2(M - base);
+    num *= so;
+    den *= so;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      // -inf: nothing; a NaN goes on.
+      const float w = laundered(x[i]) == 0xFF800000u ? 0.f : fast_exp2(x[i] - base);
+      num += o[i] * w;
+      den += w;
+    }
+    M = top;
   }
   T* o = reinterpret_cast<T*>(a.out) + tok * a.o_st + (r - tok * a.H) * a.o_sh + d;
   const float inv = den > 0.f ? 1.f / den : 0.f;
@@ -823,8 +852,12 @@ int64_t query_tiles(const vaa_attn_params* p, int num_tokens) {
   return (static_cast<int64_t>(num_tokens) * p->queries_per_kv + kRows - 1) / kRows;
 }
 
-// Workgroups over the keys: as many as fill the two slots of every CU, each with at
-// least kMinSplitTiles tiles of the longest context.
+// Workgroups over the keys: as many as fill the two slots of every CU, but no more
+// than pay.  n splits of T tiles cost T / n tiles and n times the rows' partials, B
+// bytes; the sum is least at n^2 = T kTileBytes / B.  Measured (whole call, heads 32 on 8
+// of 128 unless said): 64 tokens over 4000 15 splits 30.1 us, 31 37.5 us; over 1000 4
+// splits 24.4, 8 23.2, 17 28.7 us; 5 tokens over 4000 15 splits 22.0, 31 20.2, 63 22.3
+// us; 8 x 5 tokens over 1000, heads 14 on 2 of 64: 4 splits 49.0, 16 23.9 us.
 int plan_splits(const vaa_attn_params* p, const vaa_kv_view* view, int num_tokens) {
   const int64_t wgs = query_tiles(p, num_tokens) * p->num_kv_heads;
   const int64_t cap = static_cast<int64_t>(p->max_blocks_per_seq) * p->block_size;
@@ -835,7 +868,12 @@ int plan_splits(const vaa_attn_params* p, const vaa_kv_view* view, int num_token
   const int64_t tiles = (len + kKT - 1) / kKT;
   const int64_t slots = 2 * num_cus();
   int64_t n = wgs > 0 ? slots / wgs : 1;
-  n = std::min<int64_t>({n, tiles / kMinSplitTiles, kMaxSplits});
+  const int64_t bytes = static_cast<int64_t>(num_tokens) * p->num_query_heads *
+                        padded_head(p->head_size) * sizeof(float);
+  n = std::min<int64_t>({n, tiles, kMaxSplits});
+  if (n > 1)
+    n = std::min(n, static_cast<int64_t>(std::sqrt(static_cast<double>(tiles * kTileBytes) /
+                                                   static_cast<double>(bytes))));
   return static_cast<int>(std::max<int64_t>(1, n));
 }
 
