@@ -464,10 +464,11 @@ int vaa_kv_read_slots_q8(const vaa_attn_params* p, const vaa_kv_view* view,
  * (there is no fused write).  Arguments, guards and workspace as there, with two
  * differences: partition_size > 0 and the automatic one count the tokens that
  * are seen, and VAA_PARTITION_BALANCED_SHARED is VAA_ERR_UNSUPPORTED.
- * p->scale must be positive.  VAA_CACHE_E4M3: head_size a multiple of 16, codes
- * 16-byte aligned with strides that are multiples of 16; K, Q and V enter the products as p->dtype, which holds
- * every value of a row written from it exactly (fp16: but for those below its
- * normal range).
+ * p->scale must be positive and finite, and a block below 2^31 values.
+ * VAA_CACHE_E4M3: head_size a multiple of 16, codes 16-byte aligned with strides that
+ * are multiples of 16; K, Q and V enter the products as p->dtype, which holds every
+ * value of a row written from it exactly (fp16: but for those below its normal
+ * range).
  */
 size_t vaa_paged_attention_decode_view_workspace_size(const vaa_attn_params* p,
                                                       const vaa_kv_view* view,
@@ -487,7 +488,9 @@ int vaa_paged_attention_decode_view(const vaa_attn_params* p, const vaa_kv_view*
  * the keys over workgroups and merge (a second launch); workspace:
  * vaa_paged_attention_prefill_view_workspace_size bytes (0: none), 16-byte aligned,
  * not shared by calls that can run concurrently.  p->max_seq_len bounds the
- * contexts (it only sizes the split).  VAA_CACHE_E4M3 as for the decode.
+ * contexts (it only sizes the split).  Scale, blocks and VAA_CACHE_E4M3 as for the
+ * decode, but V enters its product in fp16, relative to the largest exponent of
+ * the rows seen so far: exact but for values 2^14 below those.
  */
 size_t vaa_paged_attention_prefill_view_workspace_size(const vaa_attn_params* p,
                                                        const vaa_kv_view* view, int num_tokens);
