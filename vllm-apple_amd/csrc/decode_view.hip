@@ -19,6 +19,13 @@
 //    MFMAs; the stream hides them), for fp16 2^8 above its softmax value so that the
 //    lo half stays a normal number down to 2^-10.  One rounding of P would cost as
 //    much as the rounding of the output itself.
+//
+// Measured (heads 32 on 8 of 128, blocks of 16): 32 contexts of 8192, e4m3 93 us, 5.8
+// TB/s (a kernel that only reads the rows 80.5; the 16-bit decode of them 162); windows of
+// 4096 and 4 first tokens, 27 sequences of 16-bit rows 87 us (75 only read), 64 of e4m3
+// rows 117 us with the merge (95).  A wave's tile is a chain (wait, convert, QK, softmax,
+// PV) at two waves a SIMD: taking the exponents away, or three tiles ahead, changed
+// nothing.
 #include "fp8.h"
 #include "kv_view.h"
 
@@ -38,10 +45,18 @@ constexpr float kPShift<bf16> = 0.f;
 constexpr int kQuantum = 128;     // fixed partitions: a multiple of this many tokens
 constexpr int kWideWaves = 8;     // waves of a workgroup with a long partition
 constexpr int kWaves4 = 4;        // ... with a short one, and of the balanced split
-constexpr int kShortTokens = 1024;
-constexpr int kBalPerCu = 2;      // balanced: workgroups per CU's worth
-constexpr int kBalMinTiles = 32;  // least share of a workgroup
-constexpr int kSeqTiles = 8;      // a sequence's start-up, in tiles
+// Partitions up to this long take four waves.  Eight against four, us (heads 32 on 8 of
+// 128): 32 x 8192 e4m3 in partitions of 512 199 / 138, of 2048 118 / 102; 8 x 32768 in
+// 2048 16-bit 180 / 170, in 4096 e4m3 112 / 105, 16-bit 170 / 165.  Longer ones are few:
+// 4 x 32768 e4m3, heads 16 on 4, in 4096 50 / 50, in 8192 78 / 85.
+constexpr int kShortTokens = 4096;
+// Balanced: workgroups per CU's worth.  1, 2, 3: 27 ragged contexts of 100 to 9000, e4m3
+// 65, 59, 73 us; 64 windows of 4096 128, 117, 122 us.
+constexpr int kBalPerCu = 2;
+// Balanced: least share of a workgroup.  8 x 2048 e4m3 32 us at 32 tiles, 20 at 8.
+constexpr int kBalMinTiles = 8;
+// Balanced: a sequence's start-up, in tiles.  2, 8: 27 ragged contexts 62, 59 us.
+constexpr int kSeqTiles = 8;
 constexpr int kBalMaxSeqs = 8192;
 
 struct Args {
@@ -836,7 +851,7 @@ int launch(const Args& a0, const Split& sp, hipStream_t stream) {
     return check_launch("decode_view_merge_kernel");
   }
   const dim3 grid(a.kvh * a.chunks, a.max_parts, a.num_seqs);
-  if (a.max_parts > 1 && sp.part <= kShortTokens * (Q8 ? 2 : 1))
+  if (a.max_parts > 1 && sp.part <= kShortTokens)
     hipLaunchKernelGGL((decode_view_kernel<D, T, Q8, kWaves4, kAny>), grid,
                        dim3(kWaves4 * kWave), lds(kWaves4), stream, a);
   else
